@@ -286,9 +286,10 @@ def exact(case, seed):
     for r in range(0, case["rows"], rows_at_once):
         x = state["x"][r:r + rows_at_once].double()
         tokens = state["tokens"][r:r + rows_at_once]
-        z = torch.logsumexp(x, 1)
-        nothing = z == -math.inf
-        logp = torch.where(nothing[:, None], -math.inf, x - torch.where(nothing, 0.0, z)[:, None])
+        m = x.amax(1, keepdim=True)
+        nothing = m == -math.inf
+        t = x - torch.where(nothing, 0.0, m)  # before the logarithm: beside a mask of the type's lowest value that would be lost
+        logp = t - torch.where(nothing, 1.0, t.exp().sum(1, keepdim=True)).log()
         p = logp.exp()
         h = -torch.where(p > 0, p * logp, torch.zeros_like(p)).sum(1)
         given = logp.gather(1, tokens.clamp(min=0)[:, None]).squeeze(1)
