@@ -305,6 +305,57 @@ int small_b200_conv_weights_prepare_f32(int32_t K_padded, int32_t K_effective, i
                                         const float *bn_running_var, float bn_eps, float *packed_filters,
                                         float *packed_bias, void *stream);
 
+/* ---- narrow types: 8-bit floating point with block scales, 16-bit floats -------------- */
+/* Element types of the layers below.  The reference has fp32 and uint8 buffers only; none of these layers has a counterpart in it. */
+enum
+{
+    SMALL_B200_TYPE_F32 = 0,
+    SMALL_B200_TYPE_BF16 = 1,
+    SMALL_B200_TYPE_F16 = 2
+};
+/* A matrix [rows][columns] to e4m3 codes with one fp32 scale for each block of 128 columns by `block_rows` rows (1: activations,
+ * 128: weights); the last blocks may be cut short.
+ *   scale = max|x| / 448 rounded to fp32, at least 2^-126; 1 for a block of zeros
+ *   code  = x / scale (the exact quotient) to the nearest e4m3 value, ties to even; x stands for code * scale
+ * NaN and infinities become NaN and take no part in the scale.
+ *   in      rows of in_type, in_stride elements apart (0 = packed)
+ *   out     [rows][columns] bytes, on a 16-byte boundary
+ *   scales  [rows or ceil(rows / 128)][ceil(columns / 128)]
+ * columns % 16 == 0; fewer than 2^31 blocks. */
+int small_b200_quantize_blocks_f8(int32_t rows, int32_t columns, int32_t block_rows, int32_t in_type, const void *in, int64_t in_stride,
+                                  void *out, float *scales, void *stream);
+/* A dense layer on such operands (small::Dense, interface_abstract.hpp:2113, on 8-bit floats):
+ *   out[r][k] = act(out[r][k] (accumulate) + bias[k] + sum over blocks b of in_scales[r][b] * filt_scales[k / 128][b] * dot of the block),
+ * products and sums in fp32, one rounding to out_type at the end (with accumulate, after adding to what is there).
+ *   in    [rows][C] e4m3, scales [rows][ceil(C / 128)]          filt  [K][C] e4m3, scales [ceil(K / 128)][ceil(C / 128)]
+ *   bias  [K] fp32 or NULL                                      out   [rows][K] of out_type
+ * Strides are in elements between rows, 0 = packed; what lies between the K outputs of two rows is left as it is.  C % 16 == 0, in and filt on
+ * 16-byte boundaries with strides that are multiples of 16.  The product of two scales is rounded to fp32, so it should be a normal number. */
+typedef struct small_b200_dense
+{
+    int32_t rows, K, C;
+    int32_t out_type;   /* SMALL_B200_TYPE_* */
+    int64_t in_stride, filt_stride, out_stride;
+    int32_t accumulate; /* 1 = start from the existing output, as the Partial* forms do */
+    int32_t act;        /* SMALL_B200_ACT_* */
+    float slope;
+} small_b200_dense;
+int small_b200_dense_f8(const small_b200_dense *D, const void *in, const float *in_scales, const void *filt, const float *filt_scales,
+                        const float *bias, void *out, void *stream);
+/* What a model answers with: for each row of logits the log-probability of a given class, the entropy of the distribution and its `top` best
+ * classes with their log-probabilities, in one pass.  Everything is computed in fp32.
+ *   logits        rows of in_type, `stride` elements apart (0 = packed)
+ *   tokens        [rows] the given classes, whole numbers of token_bytes (4 or 8) bytes; a negative one means that none is given and gives a
+ *                 log-probability of 0, one that is not below `classes` gives NaN
+ *   logprobs      [rows], entropy [rows] (natural units), top_logprobs / top_tokens [rows][top] in descending order, of equal logits the lowest
+ *                 class first.  Each may be NULL; top <= 32 and <= classes.
+ * Classes at minus infinity are masked; a row with nothing else has log-probabilities of minus infinity and an entropy of 0.  A row with NaN or
+ * plus infinity has no distribution: its log-probabilities and entropy are NaN, and NaN ranks with minus infinity.
+ * (small::SoftMax, interface_abstract.hpp:1778, has no maximum subtraction and no classes to choose.) */
+int small_b200_logprobs(int32_t rows, int32_t classes, int32_t in_type, const void *logits, int64_t stride, int32_t token_bytes,
+                        const void *tokens, float *logprobs, float *entropy, int32_t top, float *top_logprobs, int32_t *top_tokens,
+                        void *stream);
+
 /* ---- detection head ---------------------------------------------------------------- */
 /* small::YOLOLayer::compute_output (include/small/YOLOLayer.hpp:96-222): the packed activation
  * [N][C_padded/16][H][W][16], read as [anchor][5 + classes][H][W], becomes one record

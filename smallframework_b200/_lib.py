@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(PKG, "lib", "libsmall_b200.so")
 
 OK, INVALID_ARGUMENT, CUDA_ERROR, OUT_OF_MEMORY, DEVICE_TIMEOUT = range(5)
 ACT_NONE, ACT_RELU, ACT_LEAKY = 0, 1, 2
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 
 
 class Layer(C.Structure):
@@ -27,6 +28,13 @@ class Layer(C.Structure):
         ho = max((self.H + self.pad_t + self.pad_b - self.Fh) // (self.stride_h or self.stride) + 1, 0)
         wo = max((self.W + self.pad_l + self.pad_r - self.Fw) // self.stride + 1, 0)
         return ho, wo
+
+
+class DenseLayer(C.Structure):
+    """small_b200_dense"""
+    _fields_ = [("rows", C.c_int32), ("K", C.c_int32), ("C", C.c_int32), ("out_type", C.c_int32),
+                ("in_stride", C.c_int64), ("filt_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("accumulate", C.c_int32), ("act", C.c_int32), ("slope", C.c_float)]
 
 
 class SmallB200Error(RuntimeError):
@@ -99,6 +107,9 @@ SIGNATURES = {
     "small_b200_conv_weights_prepare_f32": [_I32, _I32, _I32, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _F, _VP, _VP, _VP],
     "small_b200_yolo_decode_f32": [_I32, _I32, _I32, _I32, _I32, _I32, _F, _VP, _VP, _VP, _VP],
     "small_b200_nms_f32": [_VP, _I32, _I32, _F, _F, _I32, _VP, _I32, _VP, _VP, _VP],
+    "small_b200_quantize_blocks_f8": [_I32, _I32, _I32, _I32, _VP, _I64, _VP, _VP, _VP],
+    "small_b200_dense_f8": [C.POINTER(DenseLayer), _VP, _VP, _VP, _VP, _VP, _VP, _VP],
+    "small_b200_logprobs": [_I32, _I32, _I32, _VP, _I64, _I32, _VP, _VP, _VP, _I32, _VP, _VP, _VP],
     "small_b200_conv2d_u8": [_LP, _VP, _VP, _VP, _VP, _VP],
     "small_b200_conv2d_u8_cuda_cores": [_LP, _VP, _VP, _VP, _VP, _VP],
     "small_b200_conv2d_u8_tensor_core": [_LP, _VP, _VP, _VP, _VP, _VP],

@@ -1,0 +1,621 @@
+// dense_f8.cu -- dense layer on e4m3 operands with an fp32 scale for each block of 128 (one row of activations, 128 rows of weights), on the tensor
+// cores (tcgen05 kind::f8f6f4).
+//
+// Mathematics: out[r][k] = sum_b sx[r][b] * sw[k / 128][b] * d_b, d_b the dot product of block b.  A block is 128 bytes of a row, one
+// 128-byte swizzle row in shared memory and four MMAs of 32 steps; its sums go to tensor memory by themselves, and the warps behind fold them into
+// fp32 registers, times the two scales.  Tensor memory holds several blocks' sums, so that the next MMAs run meanwhile.
+//
+// Two kernels:
+//   few    weights are the 128 lanes, 16 to 128 rows of activations the columns.  The weights' bytes bound it: they come once, by TMA, into all SMs,
+//          the reduction cut among the CTAs of a cluster where output tiles are few; the parts are added over distributed shared memory, in order.
+//   many   128 rows of activations are the lanes, 256 outputs the columns.  The tensor cores bound it; one CTA an SM takes tile after tile.
+#include <algorithm>
+
+#include "narrow_types.cuh"
+#include "tc_common.cuh"
+
+namespace
+{
+using namespace sb;
+
+constexpr int KB = 128, A_BYTES = 128 * KB;
+
+struct DenseArgs
+{
+    int rows, K, blocks; // blocks of 128 in the reduction
+    int k_tiles, r_tiles, split;
+    int accumulate;
+    float neg_scale;
+    long long out_stride;
+    const float *in_scales, *filt_scales, *bias;
+    void *out;
+    int wide; // rows of the output begin on 16-byte boundaries
+};
+
+// ReLU and LeakyReLU of the finished sum; unlike the convolutions' branch-free form exact for infinities too.
+__device__ __forceinline__ float activate(float v, float neg_scale) { return v > 0.f || neg_scale == 1.f ? v : (neg_scale == 0.f ? (v != v ? v : 0.f) : v * neg_scale); }
+
+template <int TYPE>
+__device__ __forceinline__ void store1(void *p, long long at, float v)
+{
+    if (TYPE == SMALL_B200_TYPE_F32)
+        static_cast<float *>(p)[at] = v;
+    else if (TYPE == SMALL_B200_TYPE_BF16)
+        static_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v);
+    else
+        static_cast<__half *>(p)[at] = __float2half_rn(v);
+}
+
+// The four MMAs of one block: both operands K-major with 128-byte swizzle, eight rows 1024 bytes apart.
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t sa, uint32_t sb_, uint32_t idesc)
+{
+#pragma unroll
+    for (int k = 0; k < KB / 32; ++k)
+        tc_mma_f8(d, make_smem_desc(sa + 32 * k, 16, 1024, 2), make_smem_desc(sb_ + 32 * k, 16, 1024, 2), idesc, k > 0 ? 1u : 0u);
+}
+
+__device__ __forceinline__ uint8_t *align1024(uint8_t *p) { return p + ((1024u - (smem_u32(p) & 1023u)) & 1023u); }
+
+// ------------------------------------------------------------------------------------------------ few rows
+template <int BN>
+struct Few
+{
+    static constexpr int STAGE = A_BYTES + BN * KB, STAGES = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
+    static constexpr int BUFS = BN == 128 ? 2 : 4, COLS = BUFS * BN;
+    static constexpr int CHUNK = 8; // blocks whose scales are brought at a time
+    static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * CHUNK * BN * 4;
+    static_assert(STAGES * STAGE >= BN * 128 * 4, "the ring holds the sums that a cluster adds");
+};
+constexpr int FEW_THREADS = 7 * 32;
+
+template <int BN, int TYPE>
+__global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                                      const DenseArgs a, int *status)
+{
+    using G = Few<BN>;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t full[G::STAGES], empty[G::STAGES], sum_full[G::BUFS], sum_empty[G::BUFS], sc_full[2], sc_empty[2], drained;
+    __shared__ uint32_t tmem_s;
+    uint8_t *ring = align1024(raw);
+    float *scales = reinterpret_cast<float *>(ring + G::STAGES * G::STAGE); // [2][CHUNK][BN]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = (int)(blockIdx.x % a.split), tile = (int)(blockIdx.x / a.split);
+    const int kt = tile % a.k_tiles, r0 = tile / a.k_tiles * BN;
+    const int share = (a.blocks + a.split - 1) / a.split;
+    const int b0 = rank * share, n = max(0, min(a.blocks, b0 + share) - b0);
+
+    if (tid == 0)
+    {
+        for (int s = 0; s < G::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < G::BUFS; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], 4); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&sc_full[s], 1); mbar_init(&sc_empty[s], 4); }
+        mbar_init(&drained, 1);
+        fence_barrier_init();
+    }
+    if (warp == 5)
+    {
+        tmem_alloc(&tmem_s, G::COLS < 32 ? 32 : G::COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = tmem_s;
+    float acc[BN];
+
+    if (warp < 4)
+    {
+        // ---- thread = one output channel: folds every block's sums into registers
+#pragma unroll
+        for (int c = 0; c < BN; ++c)
+            acc[c] = 0.f;
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i)
+        {
+            const int buf = i % G::BUFS, chunk = i / G::CHUNK;
+            if (i % G::CHUNK == 0)
+                ok = mbar_wait(&sc_full[chunk & 1], (chunk >> 1) & 1, status, 101);
+            ok = ok && mbar_wait(&sum_full[buf], (i / G::BUFS) & 1, status, 102);
+            if (!__all_sync(0xffffffffu, ok))
+            {
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(buf * BN);
+            const float4 *s4 = reinterpret_cast<const float4 *>(scales + ((chunk & 1) * G::CHUNK + i % G::CHUNK) * BN);
+            constexpr int STEP = BN < 32 ? 16 : 32;
+#pragma unroll
+            for (int c0 = 0; c0 < BN; c0 += STEP)
+            {
+                uint32_t r[STEP];
+                if (STEP == 32)
+                    tmem_ld32(from + c0, r);
+                else
+                    tmem_ld16(from + c0, r);
+                tmem_ld_wait();
+                if (c0 + STEP == BN)
+                {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&sum_empty[buf]);
+                }
+#pragma unroll
+                for (int c = 0; c < STEP; c += 4)
+                {
+                    const float4 s = s4[(c0 + c) / 4];
+                    acc[c0 + c] = fmaf(__uint_as_float(r[c]), s.x, acc[c0 + c]);
+                    acc[c0 + c + 1] = fmaf(__uint_as_float(r[c + 1]), s.y, acc[c0 + c + 1]);
+                    acc[c0 + c + 2] = fmaf(__uint_as_float(r[c + 2]), s.z, acc[c0 + c + 2]);
+                    acc[c0 + c + 3] = fmaf(__uint_as_float(r[c + 3]), s.w, acc[c0 + c + 3]);
+                }
+            }
+            if (i % G::CHUNK == G::CHUNK - 1)
+            {
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&sc_empty[chunk & 1]);
+            }
+        }
+    }
+    else if (warp == 4)
+    {
+        if (lane == 0)
+        {
+            bool ok = true;
+            int i = 0;
+            for (; i < n; ++i)
+            {
+                const int s = i % G::STAGES;
+                if (i >= G::STAGES && !mbar_wait(&empty[s], (i / G::STAGES - 1) & 1, status, 103))
+                {
+                    ok = false;
+                    break;
+                }
+                mbar_expect_tx(&full[s], G::STAGE);
+                tma_load_2d(ring + s * G::STAGE, &map_w, (b0 + i) * KB, kt * 128, &full[s]);
+                tma_load_2d(ring + s * G::STAGE + A_BYTES, &map_x, (b0 + i) * KB, r0, &full[s]);
+            }
+            for (int j = max(0, i - G::STAGES); j < i && !ok; ++j) // its own copies in flight
+                mbar_wait(&full[j % G::STAGES], (j / G::STAGES) & 1, status, 104);
+        }
+    }
+    else if (warp == 5)
+    {
+        if (lane == 0)
+        {
+            const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 128, BN);
+            bool ok = true;
+            for (int i = 0; i < n && ok; ++i)
+            {
+                const int s = i % G::STAGES, buf = i % G::BUFS;
+                ok = mbar_wait(&full[s], (i / G::STAGES) & 1, status, 105) &&
+                     (i < G::BUFS || mbar_wait(&sum_empty[buf], (i / G::BUFS - 1) & 1, status, 106));
+                if (!ok)
+                    break;
+                tc_fence_after_sync();
+                const uint32_t sa = smem_u32(ring + s * G::STAGE);
+                mma_block(tmem + (uint32_t)(buf * BN), sa, sa + A_BYTES, idesc);
+                tc_commit(&empty[s]);
+                tc_commit(&sum_full[buf]);
+            }
+            if (!ok)
+            {
+                tc_commit(&drained);
+                mbar_wait(&drained, 0, status, 107);
+            }
+        }
+    }
+    else
+    {
+        // ---- scales: the product of a row's and the weights' scale, by block and row
+        constexpr int ROWS = (BN + 31) / 32;
+        const int chunks = (n + G::CHUNK - 1) / G::CHUNK;
+        const float *sw = a.filt_scales + (size_t)kt * a.blocks + b0;
+        for (int c = 0; c < chunks; ++c)
+        {
+            float v[ROWS][G::CHUNK];
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q)
+            {
+                const int col = q * 32 + lane, row = r0 + col;
+                const float *sx = a.in_scales + (size_t)row * a.blocks + b0;
+#pragma unroll
+                for (int j = 0; j < G::CHUNK; ++j)
+                {
+                    const int b = c * G::CHUNK + j;
+                    v[q][j] = col < BN && row < a.rows && b < n ? __ldg(sx + b) * __ldg(sw + b) : 0.f;
+                }
+            }
+            bool ok = c < 2 || mbar_wait(&sc_empty[c & 1], ((c >> 1) - 1) & 1, status, 108);
+            if (!__all_sync(0xffffffffu, ok))
+                break;
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+                for (int j = 0; j < G::CHUNK; ++j)
+                    if (q * 32 + lane < BN)
+                        scales[((c & 1) * G::CHUNK + j) * BN + q * 32 + lane] = v[q][j];
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&sc_full[c & 1]);
+        }
+    }
+    __syncwarp();
+
+    // ---- the cluster's parts, then bias, activation and the one rounding
+    const int k = kt * 128 + tid;
+    auto finish = [&](int col, float v) {
+        const int row = r0 + col;
+        if (row >= a.rows || k >= a.K)
+            return;
+        const long long at = (long long)row * a.out_stride + k;
+        if (a.accumulate)
+            v += load1<TYPE>(a.out, at);
+        if (a.bias)
+            v += __ldg(a.bias + k);
+        store1<TYPE>(a.out, at, activate(v, a.neg_scale));
+    };
+    if (a.split == 1)
+    {
+        if (warp < 4)
+        {
+#pragma unroll
+            for (int c = 0; c < BN; ++c)
+                finish(c, acc[c]);
+        }
+    }
+    else
+    {
+        float *red = reinterpret_cast<float *>(ring); // [BN][128]
+        if (warp < 4)
+        {
+#pragma unroll
+            for (int c = 0; c < BN; ++c)
+                red[c * 128 + tid] = acc[c];
+        }
+        cluster_sync_all();
+        if (warp < 4)
+        {
+            const int per = BN / a.split;
+            for (int c = rank * per; c < rank * per + per && r0 + c < a.rows; ++c)
+            {
+                float v = 0.f;
+                for (int q = 0; q < a.split; ++q)
+                {
+                    float p;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p) : "r"(map_to_cta(red + c * 128 + tid, q)));
+                    v += p;
+                }
+                finish(c, v);
+            }
+        }
+        __syncwarp();
+        cluster_sync_all(); // nobody's shared memory goes while it is read
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 5)
+        tmem_dealloc(tmem, G::COLS < 32 ? 32 : G::COLS);
+}
+
+// ------------------------------------------------------------------------------------------------ many rows
+constexpr int MANY_N = 256, MANY_STAGE = A_BYTES + MANY_N * KB, MANY_STAGES = 4, MANY_EPI = 8, MANY_THREADS = (MANY_EPI + 2) * 32;
+constexpr int MANY_SMEM = 1024 + MANY_STAGES * MANY_STAGE;
+constexpr int GROUP = 16; // tiles of rows that are walked together: their activations and the weights beside them stay in L2
+
+struct TileAt
+{
+    int r0, k0;
+};
+__device__ __forceinline__ TileAt tile_at(const DenseArgs &a, int t)
+{
+    const int per_group = GROUP * a.k_tiles, g = t / per_group, in = t - g * per_group;
+    const int size = min(GROUP, a.r_tiles - g * GROUP);
+    const int kt = in / size;
+    return {(g * GROUP + in - kt * size) * 128, kt * MANY_N};
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                                                                          const DenseArgs a, int *status)
+{
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t full[MANY_STAGES], empty[MANY_STAGES], sum_full[2], sum_empty[2], drained;
+    __shared__ uint32_t tmem_s;
+    uint8_t *ring = align1024(raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tiles = a.k_tiles * a.r_tiles;
+    if (tid == 0)
+    {
+        for (int s = 0; s < MANY_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], MANY_EPI); }
+        mbar_init(&drained, 1);
+        fence_barrier_init();
+    }
+    if (warp == MANY_EPI + 1)
+    {
+        tmem_alloc(&tmem_s, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = tmem_s;
+
+    if (warp < MANY_EPI)
+    {
+        // ---- thread = one row of activations and 128 outputs, a block of weights
+        const int half = warp >> 2, lane_row = (warp & 3) * 32 + lane;
+        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * 128);
+        bool ok = true;
+        unsigned i = 0;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+        {
+            const TileAt at = tile_at(a, t);
+            const int row = at.r0 + lane_row, k0 = at.k0 + half * 128;
+            const float *sx = a.in_scales + (size_t)min(row, a.rows - 1) * a.blocks;
+            const float *sw = a.filt_scales + (size_t)min(k0 / 128, (a.K - 1) / 128) * a.blocks;
+            float acc[128];
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+                acc[c] = 0.f;
+            float next = __ldg(sx) * __ldg(sw);
+            for (int b = 0; b < a.blocks; ++b, ++i)
+            {
+                const int buf = i & 1;
+                const float s = next;
+                if (b + 1 < a.blocks)
+                    next = __ldg(sx + b + 1) * __ldg(sw + b + 1);
+                ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[buf], (i >> 1) & 1, status, 111));
+                if (!ok)
+                    break;
+                tc_fence_after_sync();
+#pragma unroll
+                for (int c0 = 0; c0 < 128; c0 += 32)
+                {
+                    uint32_t r[32];
+                    tmem_ld32(from + (uint32_t)(buf * MANY_N + c0), r);
+                    tmem_ld_wait();
+                    if (c0 == 96)
+                    {
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0)
+                            mbar_arrive(&sum_empty[buf]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        acc[c0 + c] = fmaf(__uint_as_float(r[c]), s, acc[c0 + c]);
+                }
+            }
+            if (!ok)
+                break;
+            if (row < a.rows)
+            {
+                const long long base = (long long)row * a.out_stride + k0;
+                constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE;
+#pragma unroll
+                for (int c0 = 0; c0 < 128; c0 += VE)
+                {
+                    if (k0 + c0 >= a.K)
+                        break;
+                    float v[VE];
+#pragma unroll
+                    for (int c = 0; c < VE; ++c)
+                    {
+                        v[c] = acc[c0 + c];
+                        if (k0 + c0 + c < a.K)
+                        {
+                            if (a.accumulate)
+                                v[c] += load1<TYPE>(a.out, base + c0 + c);
+                            if (a.bias)
+                                v[c] += __ldg(a.bias + k0 + c0 + c);
+                            v[c] = activate(v[c], a.neg_scale);
+                        }
+                    }
+                    if (a.wide && k0 + c0 + VE <= a.K)
+                    {
+                        uint4 w;
+                        if (TYPE == SMALL_B200_TYPE_F32)
+                            w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                        else
+                            w = make_uint4(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]), pack2<TYPE>(v[VE - 4], v[VE - 3]),
+                                           pack2<TYPE>(v[VE - 2], v[VE - 1]));
+                        *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + (base + c0) * SIZE) = w;
+                    }
+                    else
+                    {
+#pragma unroll
+                        for (int c = 0; c < VE; ++c)
+                            if (k0 + c0 + c < a.K)
+                                store1<TYPE>(a.out, base + c0 + c, v[c]);
+                    }
+                }
+            }
+        }
+    }
+    else if (warp == MANY_EPI)
+    {
+        if (lane == 0)
+        {
+            bool ok = true;
+            unsigned i = 0;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+            {
+                const TileAt at = tile_at(a, t);
+                for (int b = 0; b < a.blocks; ++b, ++i)
+                {
+                    const unsigned s = i % MANY_STAGES;
+                    if (i >= MANY_STAGES && !mbar_wait(&empty[s], (i / MANY_STAGES - 1) & 1, status, 112))
+                    {
+                        ok = false;
+                        break;
+                    }
+                    mbar_expect_tx(&full[s], MANY_STAGE);
+                    tma_load_2d(ring + s * MANY_STAGE, &map_x, b * KB, at.r0, &full[s]);
+                    tma_load_2d(ring + s * MANY_STAGE + A_BYTES, &map_w, b * KB, at.k0, &full[s]);
+                }
+            }
+            for (unsigned j = i > MANY_STAGES ? i - MANY_STAGES : 0; j < i && !ok; ++j) // its own copies in flight
+                mbar_wait(&full[j % MANY_STAGES], (j / MANY_STAGES) & 1, status, 113);
+        }
+    }
+    else if (lane == 0)
+    {
+        const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 128, MANY_N);
+        bool ok = true;
+        unsigned i = 0;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+            for (int b = 0; b < a.blocks; ++b, ++i)
+            {
+                const unsigned s = i % MANY_STAGES, buf = i & 1;
+                ok = mbar_wait(&full[s], (i / MANY_STAGES) & 1, status, 114) &&
+                     (i < 2 || mbar_wait(&sum_empty[buf], ((i >> 1) - 1) & 1, status, 115));
+                if (!ok)
+                    break;
+                tc_fence_after_sync();
+                const uint32_t sa = smem_u32(ring + s * MANY_STAGE);
+                mma_block(tmem + buf * MANY_N, sa, sa + A_BYTES, idesc);
+                tc_commit(&empty[s]);
+                tc_commit(&sum_full[buf]);
+            }
+        if (!ok)
+        {
+            tc_commit(&drained);
+            mbar_wait(&drained, 0, status, 116);
+        }
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == MANY_EPI + 1)
+        tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int map_rows(CUtensorMap *map, const void *p, int rows, int C, long long stride, int box_rows)
+{
+    const uint64_t dims[2] = {(uint64_t)C, (uint64_t)rows}, strides[1] = {(uint64_t)stride};
+    const uint32_t box[2] = {KB, (uint32_t)box_rows};
+    return make_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int BN, int TYPE>
+int launch_few(DenseArgs a, const CUtensorMap &map_w, const CUtensorMap &map_x, int *status, cudaStream_t st)
+{
+    using G = Few<BN>;
+    auto kern = dense_f8_few_kernel<BN, TYPE>;
+    static PerDeviceOnce configured;
+    int dev;
+    if (configured.needed(&dev))
+    {
+        SB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+        configured.mark(dev);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.k_tiles * a.r_tiles * a.split));
+    cfg.blockDim = dim3(FEW_THREADS);
+    cfg.dynamicSmemBytes = G::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SB_CUDA(cudaLaunchKernelEx(&cfg, kern, map_w, map_x, a, status));
+    return launched("dense_f8_few_kernel");
+}
+
+template <int TYPE>
+int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long in_stride, const void *filt, long long filt_stride, cudaStream_t st)
+{
+    int *status = device_status_ptr();
+    if (!status)
+        return fail(SMALL_B200_CUDA_ERROR, "device status word not available");
+    CUtensorMap map_w, map_x;
+    if (D->rows <= 128)
+    {
+        const int bn = D->rows <= 16 ? 16 : D->rows <= 32 ? 32 : D->rows <= 64 ? 64 : 128;
+        a.k_tiles = (D->K + 127) / 128;
+        a.r_tiles = (D->rows + bn - 1) / bn;
+        // Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each at least two blocks.
+        a.split = 1;
+        while (a.split < 8 && (long long)a.k_tiles * a.r_tiles * a.split * 2 <= 2LL * num_sms() && a.blocks >= 4 * a.split)
+            a.split *= 2;
+        if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, 128))
+            return rc;
+        if (int rc = map_rows(&map_x, in, D->rows, D->C, in_stride, bn))
+            return rc;
+        switch (bn)
+        {
+        case 16: return launch_few<16, TYPE>(a, map_w, map_x, status, st);
+        case 32: return launch_few<32, TYPE>(a, map_w, map_x, status, st);
+        case 64: return launch_few<64, TYPE>(a, map_w, map_x, status, st);
+        default: return launch_few<128, TYPE>(a, map_w, map_x, status, st);
+        }
+    }
+    a.k_tiles = (D->K + MANY_N - 1) / MANY_N;
+    a.r_tiles = (D->rows + 127) / 128;
+    a.split = 1;
+    if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, MANY_N))
+        return rc;
+    if (int rc = map_rows(&map_x, in, D->rows, D->C, in_stride, 128))
+        return rc;
+    auto kern = dense_f8_many_kernel<TYPE>;
+    static PerDeviceOnce configured;
+    int dev;
+    if (configured.needed(&dev))
+    {
+        SB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MANY_SMEM));
+        configured.mark(dev);
+    }
+    const int tiles = a.k_tiles * a.r_tiles;
+    kern<<<std::min(tiles, num_sms()), MANY_THREADS, MANY_SMEM, st>>>(map_x, map_w, a, status);
+    return launched("dense_f8_many_kernel");
+}
+} // namespace
+
+extern "C" int small_b200_dense_f8(const small_b200_dense *D, const void *in, const float *in_scales, const void *filt, const float *filt_scales,
+                                   const float *bias, void *out, void *stream)
+{
+    const std::string name = "Dense<float8>";
+    if (!D)
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: null layer.");
+    if (D->C <= 0 || D->C % CB != 0)
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: in_channels unsupported.");
+    if (D->K <= 0)
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: out_channels unsupported.");
+    const int size = type_size(D->out_type);
+    if (size == 0)
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: output type unsupported.");
+    if (D->act != SMALL_B200_ACT_NONE && D->act != SMALL_B200_ACT_RELU && D->act != SMALL_B200_ACT_LEAKY)
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: activation unsupported.");
+    const long long in_stride = D->in_stride ? D->in_stride : D->C, filt_stride = D->filt_stride ? D->filt_stride : D->C,
+                    out_stride = D->out_stride ? D->out_stride : D->K;
+    if (D->rows < 0 || in_stride < D->C || filt_stride < D->C || out_stride < D->K || in_stride % 16 != 0 || filt_stride % 16 != 0 ||
+        in_stride >= 1LL << 40 || filt_stride >= 1LL << 40) // what a tensor map holds
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: bad shape.");
+    if (D->rows == 0)
+        return SMALL_B200_OK;
+    if (!in || !in_scales || !filt || !filt_scales || !out)
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: null buffer.");
+    auto off = [](const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
+    if (off(in, 16) || off(filt, 16) || off(in_scales, 4) || off(filt_scales, 4) || off(bias, 4) || off(out, size))
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: misaligned buffer (operands begin on 16-byte boundaries).");
+    if (((D->K + 127LL) / 128) * ((D->rows + 15LL) / 16) * 8 > 0x7fffffffLL)
+        return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: too many tiles.");
+    DenseArgs a = {};
+    a.rows = D->rows; a.K = D->K; a.blocks = (D->C + KB - 1) / KB;
+    a.accumulate = D->accumulate; a.neg_scale = D->act == SMALL_B200_ACT_RELU ? 0.f : D->act == SMALL_B200_ACT_LEAKY ? D->slope : 1.f;
+    a.out_stride = out_stride; a.in_scales = in_scales; a.filt_scales = filt_scales; a.bias = bias; a.out = out;
+    a.wide = !off(out, 16) && out_stride * size % 16 == 0;
+    cudaStream_t st = as_stream(stream);
+    switch (D->out_type)
+    {
+    case SMALL_B200_TYPE_F32: return dispatch<SMALL_B200_TYPE_F32>(D, a, in, in_stride, filt, filt_stride, st);
+    case SMALL_B200_TYPE_BF16: return dispatch<SMALL_B200_TYPE_BF16>(D, a, in, in_stride, filt, filt_stride, st);
+    default: return dispatch<SMALL_B200_TYPE_F16>(D, a, in, in_stride, filt, filt_stride, st);
+    }
+}

@@ -1,0 +1,452 @@
+// logprobs.cu -- log-probabilities of given classes, entropy and the best alternatives of rows of logits, in one pass over them.
+//
+// Mathematics, for a row x: m = max x, t_i = x_i - m, S = sum e^t_i, T = sum t_i e^t_i;
+//   log p_i = t_i - log S,   H = -sum p_i log p_i = log S - T / S  (both terms non-negative: no cancellation).
+// Every thread keeps (m, S, T) of the vectors it has read and rescales when its maximum moves; pairs merge as S = sum S_j e^(m_j - m),
+// T = sum (T_j + S_j (m_j - m)) e^(m_j - m).  A masked class (minus infinity, or a value so low that its exponential is 0) adds 0 to both.
+//
+// Best alternatives: a thread also remembers which of its vectors first held its maximum.  These (value, vector) keys are all different, and the
+// `top` best elements lie in the `top` threads with the best keys: an element elsewhere has those threads' maxima before it.  Only these
+// threads' vectors are read again (from L2), and only elements not below the last of the keys are ranked.
+//
+// Bound: memory, every logit read once.  A row is cut among the CTAs of a cluster where rows are few, and what they found is merged over distributed
+// shared memory: no workspace, and sums are always added in the same order.
+#include <algorithm>
+
+#include "narrow_types.cuh"
+#include "tc_common.cuh"
+
+namespace
+{
+using namespace sb;
+
+constexpr int THREADS = 256, WARPS = THREADS / 32, TOP_MOST = 32, MAX_SPLIT = 8;
+constexpr int CANDIDATES = 1024;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct LogpArgs
+{
+    long long rows, stride;
+    int classes, top, split, token_bytes;
+};
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// Whole numbers in the order of the floats, all of them above 0; both zeros alike, NaN (which no maximum sees) as minus infinity.
+__device__ __forceinline__ uint32_t order_of(float x)
+{
+    x = x != x ? -INFINITY : x + 0.f;
+    const uint32_t b = __float_as_uint(x);
+    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order)
+{
+    return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
+}
+__device__ __forceinline__ unsigned long long make_key(uint32_t order, uint32_t index) { return (unsigned long long)order << 32 | (0xffffffffu - index); }
+
+struct Stats
+{
+    float m, S, T;
+};
+// Both relative to the larger maximum.
+__device__ __forceinline__ Stats merge(const Stats &a, const Stats &b)
+{
+    Stats r;
+    r.m = fmaxf(a.m, b.m);
+    r.S = r.T = 0.f;
+    if (a.m != -INFINITY || a.S != 0.f) // nothing seen there: S = T = 0
+    {
+        const float d = a.m == r.m ? 0.f : a.m - r.m, c = exp2_approx(d * LOG2E);
+        r.S += a.S * c;
+        r.T += c == 0.f ? 0.f : (a.T + a.S * d) * c;
+    }
+    if (b.m != -INFINITY || b.S != 0.f)
+    {
+        const float d = b.m == r.m ? 0.f : b.m - r.m, c = exp2_approx(d * LOG2E);
+        r.S += b.S * c;
+        r.T += c == 0.f ? 0.f : (b.T + b.S * d) * c;
+    }
+    return r;
+}
+
+// The 16 bytes of vector v of a row whose first element is element `skew` of vector 0; elements outside the row are minus infinity.
+template <int TYPE>
+__device__ __forceinline__ uint4 load_vector(const void *row, int v, int skew, int classes)
+{
+    constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8;
+    const long long first = (long long)v * VE - skew;
+    if (first >= 0 && first + VE <= classes)
+        return __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(row) + first * (16 / VE)));
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (TYPE == SMALL_B200_TYPE_F32)
+            w[i] = first + i >= 0 && first + i < classes ? static_cast<const uint32_t *>(row)[first + i] : 0xff800000u;
+        else
+        {
+            const uint32_t none = TYPE == SMALL_B200_TYPE_BF16 ? 0xff80u : 0xfc00u;
+            const long long e = first + 2 * i;
+            const uint32_t lo = e >= 0 && e < classes ? static_cast<const uint16_t *>(row)[e] : none;
+            const uint32_t hi = e + 1 >= 0 && e + 1 < classes ? static_cast<const uint16_t *>(row)[e + 1] : none;
+            w[i] = lo | hi << 16;
+        }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int TYPE>
+__device__ __forceinline__ void unpack_vector(const uint4 &w, float *x)
+{
+    if (TYPE == SMALL_B200_TYPE_F32)
+    {
+        x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
+    }
+    else
+    {
+        unpack2<TYPE>(w.x, x[0], x[1]); unpack2<TYPE>(w.y, x[2], x[3]); unpack2<TYPE>(w.z, x[4], x[5]); unpack2<TYPE>(w.w, x[6], x[7]);
+    }
+}
+
+// Descending order over the 32 lanes; FROM: the length of the bitonic runs the lanes hold already (2: none).
+template <int FROM>
+__device__ __forceinline__ unsigned long long sort_lanes(unsigned long long key, int lane)
+{
+#pragma unroll
+    for (int run = FROM; run <= 32; run <<= 1)
+#pragma unroll
+        for (int d = run >> 1; d > 0; d >>= 1)
+        {
+            const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, d);
+            const bool keep_larger = ((lane & d) == 0) == ((lane & run) == 0 || run == 32);
+            key = keep_larger == (key > other) ? key : other;
+        }
+    return key;
+}
+__device__ __forceinline__ unsigned long long block_max(unsigned long long key, unsigned long long *part)
+{
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1)
+    {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, d);
+        key = key > other ? key : other;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0)
+        part[threadIdx.x >> 5] = key;
+    __syncthreads();
+    key = part[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w)
+        key = part[w] > key ? part[w] : key;
+    return key;
+}
+
+struct Shared
+{
+    Stats part[WARPS], all;
+    unsigned long long sorted[WARPS][32];
+    unsigned long long best[TOP_MOST];                  // this CTA's best elements, in order
+    unsigned long long found[CANDIDATES];
+    unsigned long long merged[MAX_SPLIT * TOP_MOST];
+    int count;
+};
+
+template <int TYPE>
+__global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens,
+                                                            float *__restrict__ logprobs, float *__restrict__ entropy,
+                                                            float *__restrict__ top_logprobs, int *__restrict__ top_tokens)
+{
+    constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, BATCH = 4;
+    __shared__ Shared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long r = blockIdx.x / a.split;
+    const int rank = (int)(blockIdx.x % a.split);
+    const char *row = static_cast<const char *>(logits) + r * a.stride * SIZE;
+    const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / SIZE);
+    const int vectors = (int)(((long long)skew + a.classes + VE - 1) / VE);
+    const int share = (vectors + a.split - 1) / a.split;
+    const int v0 = rank * share, v1 = min(vectors, v0 + share);
+
+    // ---- one pass: maximum and sums of this thread's vectors
+    float m = -INFINITY, mu = 0.f, S = 0.f, T = 0.f; // mu: m, or 0 while there is none
+    int at = v0 + tid;                               // the vector that held m first
+    for (int v = v0 + tid; v < v1; v += BATCH * THREADS)
+    {
+        uint4 w[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (v + j * THREADS < v1)
+                w[j] = load_vector<TYPE>(row, v + j * THREADS, skew, a.classes);
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (v + j * THREADS < v1)
+            {
+                float x[VE];
+                unpack_vector<TYPE>(w[j], x);
+                float vm = x[0];
+#pragma unroll
+                for (int i = 1; i < VE; ++i)
+                    vm = fmaxf(vm, x[i]);
+                if (vm > m)
+                {
+                    if (m != -INFINITY)
+                    {
+                        const float d = m - vm, c = exp2_approx(d * LOG2E);
+                        T = c == 0.f ? 0.f : (T + S * d) * c;
+                        S *= c;
+                    }
+                    m = mu = vm;
+                    at = v + j * THREADS;
+                }
+#pragma unroll
+                for (int i = 0; i < VE; ++i)
+                {
+                    const float t = max_nan(x[i] - mu, -1e30f); // finite: the exponential's 0 times it is 0
+                    const float e = exp2_approx(t * LOG2E);
+                    S += e;
+                    T = fmaf(e, t, T);
+                }
+            }
+    }
+    const bool any = v0 + tid < v1;
+
+    // ---- the CTA's maximum and sums
+    Stats st = {m, S, T};
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1)
+    {
+        const Stats o = {__shfl_xor_sync(0xffffffffu, st.m, d), __shfl_xor_sync(0xffffffffu, st.S, d), __shfl_xor_sync(0xffffffffu, st.T, d)};
+        st = (lane & d) ? merge(o, st) : merge(st, o);
+    }
+    if (lane == 0)
+        sh.part[warp] = st;
+    if (tid == 0)
+        sh.count = 0;
+
+    if (a.top > 0)
+    {
+        // ---- the best threads
+        unsigned long long key = sort_lanes<2>(any ? make_key(order_of(m), (uint32_t)at) : 0ull, lane);
+        sh.sorted[warp][lane] = key;
+        for (int step = 1; step < WARPS; step <<= 1)
+        {
+            __syncthreads();
+            if ((warp & (2 * step - 1)) == 0)
+            {
+                const unsigned long long other = sh.sorted[warp + step][31 - lane];
+                key = sort_lanes<32>(key > other ? key : other, lane);
+                sh.sorted[warp][lane] = key;
+            }
+        }
+        __syncthreads();
+        // ---- their elements that are not below the last of them
+        const unsigned long long last = sh.sorted[0][a.top - 1];
+        const uint32_t last_order = (uint32_t)(last >> 32), last_vector = 0xffffffffu - (uint32_t)last;
+        const int per_thread = (v1 - v0 + THREADS - 1) / THREADS;
+        const bool all = last == 0ull; // fewer threads than that have any
+        auto each = [&](auto take) {
+            for (int i = tid; i < a.top * per_thread; i += THREADS)
+            {
+                const int j = i / per_thread;
+                const unsigned long long k = sh.sorted[0][j];
+                if (k == 0ull)
+                    continue;
+                const int v = v0 + (int)((0xffffffffu - (uint32_t)k - (uint32_t)v0) % THREADS) + (i - j * per_thread) * THREADS;
+                if (v >= v1)
+                    continue;
+                float x[VE];
+                unpack_vector<TYPE>(load_vector<TYPE>(row, v, skew, a.classes), x);
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                {
+                    const long long index = (long long)v * VE - skew + e;
+                    const uint32_t o = order_of(x[e]);
+                    if (index >= 0 && index < a.classes && (all || o > last_order || (o == last_order && (uint32_t)v <= last_vector)))
+                        take(make_key(o, (uint32_t)index));
+                }
+            }
+        };
+        each([&](unsigned long long k) {
+            const int n = atomicAdd(&sh.count, 1);
+            if (n < CANDIDATES)
+                sh.found[n] = k;
+        });
+        if (tid < a.top)
+            sh.best[tid] = 0ull;
+        __syncthreads();
+        const int n = sh.count;
+        if (n <= CANDIDATES)
+        {
+            for (int i = tid; i < n; i += THREADS)
+            {
+                const unsigned long long k = sh.found[i];
+                int before = 0;
+                for (int q = 0; q < n; ++q)
+                    before += sh.found[q] > k;
+                if (before < a.top)
+                    sh.best[before] = k;
+            }
+        }
+        else // rows in ascending order and the like: one after the other
+        {
+            unsigned long long limit = ~0ull;
+            for (int j = 0; j < a.top; ++j)
+            {
+                unsigned long long k = 0ull;
+                each([&](unsigned long long c) { k = c < limit && c > k ? c : k; });
+                limit = block_max(k, sh.found);
+                if (tid == 0)
+                    sh.best[j] = limit;
+                if (limit == 0ull)
+                    break;
+            }
+        }
+    }
+    __syncthreads();
+    if (tid == 0)
+    {
+        Stats s = sh.part[0];
+        for (int w = 1; w < WARPS; ++w)
+            s = merge(s, sh.part[w]);
+        sh.all = s;
+    }
+
+    // ---- the cluster's, in the first CTA
+    const unsigned long long *best = sh.best;
+    if (a.split > 1)
+    {
+        cluster_sync_all();
+        if (rank == 0)
+        {
+            if (tid == 0)
+            {
+                Stats s = sh.all;
+                for (int q = 1; q < a.split; ++q)
+                {
+                    const uint32_t p = map_to_cta(&sh.all, q);
+                    Stats o;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.m) : "r"(p));
+                    asm volatile("ld.shared::cluster.f32 %0, [%1+4];" : "=f"(o.S) : "r"(p));
+                    asm volatile("ld.shared::cluster.f32 %0, [%1+8];" : "=f"(o.T) : "r"(p));
+                    s = merge(s, o);
+                }
+                sh.all = s;
+            }
+            const int n = a.split * a.top;
+            for (int i = tid; i < n; i += THREADS)
+            {
+                unsigned long long k;
+                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(map_to_cta(&sh.best[i % a.top], i / a.top)));
+                sh.merged[i] = k;
+            }
+            __syncthreads();
+            for (int i = tid; i < n; i += THREADS)
+            {
+                const unsigned long long k = sh.merged[i];
+                int before = 0;
+                for (int q = 0; q < n; ++q)
+                    before += sh.merged[q] > k;
+                if (k != 0ull && before < a.top)
+                    sh.found[before] = k;
+            }
+            best = sh.found;
+        }
+        cluster_sync_all(); // nobody's shared memory goes while it is read
+        if (rank != 0)
+            return;
+    }
+    __syncthreads();
+
+    // ---- outputs
+    const Stats s = sh.all;
+    const bool nothing = s.m == -INFINITY && !(s.S != s.S); // every class is masked: no probability, no entropy
+    const float log_s = nothing ? 0.f : logf(s.S);
+    auto logp = [&](float x) { return nothing ? (x != x ? x : -INFINITY) : (x - s.m) - log_s; };
+    if (tid == 0)
+    {
+        if (logprobs)
+        {
+            const long long t = a.token_bytes == 8 ? static_cast<const long long *>(tokens)[r] : static_cast<const int *>(tokens)[r];
+            logprobs[r] = t < 0 ? 0.f : t >= a.classes ? NAN : logp(load1<TYPE>(row, t));
+        }
+        if (entropy)
+            entropy[r] = nothing ? 0.f : log_s - s.T / s.S;
+    }
+    if (tid < a.top)
+    {
+        const unsigned long long k = best[tid];
+        if (top_logprobs)
+            top_logprobs[r * a.top + tid] = logp(value_of((uint32_t)(k >> 32)));
+        if (top_tokens)
+            top_tokens[r * a.top + tid] = (int)(0xffffffffu - (uint32_t)k);
+    }
+}
+
+template <int TYPE>
+int launch_logprobs(const LogpArgs &a, const void *logits, const void *tokens, float *logprobs, float *entropy, float *top_logprobs,
+                    int32_t *top_tokens, cudaStream_t st)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.rows * a.split));
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SB_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<TYPE>, a, logits, tokens, logprobs, entropy, top_logprobs, (int *)top_tokens));
+    return launched("logprobs_kernel");
+}
+} // namespace
+
+extern "C" int small_b200_logprobs(int32_t rows, int32_t classes, int32_t in_type, const void *logits, int64_t stride, int32_t token_bytes,
+                                   const void *tokens, float *logprobs, float *entropy, int32_t top, float *top_logprobs, int32_t *top_tokens,
+                                   void *stream)
+{
+    const char *name = "LogProbabilities";
+    if (rows < 0 || classes <= 0 || (stride != 0 && stride < classes))
+        return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: bad shape.");
+    const int size = type_size(in_type);
+    if (size == 0)
+        return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: input type unsupported.");
+    if (token_bytes != 4 && token_bytes != 8)
+        return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: tokens are of 4 or 8 bytes.");
+    if (top < 0 || top > TOP_MOST || top > classes)
+        return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: top unsupported (at most 32, and at most the number of classes).");
+    if (rows == 0)
+        return SMALL_B200_OK;
+    if (!logits || (logprobs && !tokens))
+        return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: null buffer.");
+    if (!top_logprobs && !top_tokens)
+        top = 0;
+    if (!logprobs && !entropy && top == 0)
+        return SMALL_B200_OK;
+    auto off = [](const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
+    if (off(logits, size) || (logprobs && off(tokens, token_bytes)) || off(logprobs, 4) || off(entropy, 4) || off(top_logprobs, 4) || off(top_tokens, 4))
+        return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: misaligned buffer.");
+    LogpArgs a;
+    a.rows = rows; a.stride = stride ? stride : classes; a.classes = classes; a.top = top; a.token_bytes = token_bytes;
+    // As many CTAs to a row as fill the device twice over, while each of their threads has a vector of its own.
+    a.split = 1;
+    while (a.split < MAX_SPLIT && (long long)rows * a.split * 2 <= 2LL * num_sms() && classes / (16 / size) >= 2 * a.split * THREADS)
+        a.split *= 2;
+    if ((long long)rows * a.split > 0x7fffffffLL)
+        return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: too many rows.");
+    cudaStream_t st = as_stream(stream);
+    switch (in_type)
+    {
+    case SMALL_B200_TYPE_F32: return launch_logprobs<SMALL_B200_TYPE_F32>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st);
+    case SMALL_B200_TYPE_BF16: return launch_logprobs<SMALL_B200_TYPE_BF16>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st);
+    default: return launch_logprobs<SMALL_B200_TYPE_F16>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st);
+    }
+}

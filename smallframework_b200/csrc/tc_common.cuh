@@ -173,6 +173,13 @@ __device__ __forceinline__ void tma_load_1d(void *dst, const void *src, uint32_t
                  ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
 }
+__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int c0, int c1, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(smem_u32(bar))
+                 : "memory");
+}
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int c0, int c1, int c2,
                                             uint64_t *bar)
 {
@@ -261,7 +268,15 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t a_desc, uin
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
                  : "memory");
 }
-// The same with D = A * B + D * 2^-DOWN: what the accumulator holds is brought to another scale on the way.
+// 8-bit floating point (e4m3 with make_idesc's formats 0), fp32 accumulation, 32 reduction steps.
+__device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// Half-precision operands with D = A * B + D * 2^-DOWN: what the accumulator holds is brought to another scale on the way.
 template <int DOWN>
 __device__ __forceinline__ void tc_mma_f16_rescaled(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc)
 {
@@ -316,7 +331,7 @@ __device__ __forceinline__ uint64_t make_smem_desc(uint32_t saddr, uint32_t lbo_
 }
 
 // Instruction descriptor (32 bit): accumulator format (1 = f32, 2 = s32) at bit 4, A/B element
-// formats at bits 7 and 10 (i8 kinds: 0 = u8, 1 = s8; f16 kinds: 2 = tf32), A/B major at bits
+// formats at bits 7 and 10 (i8 kinds: 0 = u8, 1 = s8; f16 kinds: 2 = tf32; f8f6f4: 0 = e4m3), A/B major at bits
 // 15/16 (0 = K-major, 1 = MN-major), N >> 3 at bit 17, M >> 4 at bit 24.
 __host__ __device__ constexpr uint32_t make_idesc(uint32_t cfmt, uint32_t afmt, uint32_t bfmt, uint32_t a_mn,
                                                   uint32_t b_mn, uint32_t M, uint32_t N)

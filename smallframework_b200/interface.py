@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import ACT_LEAKY, ACT_NONE, ACT_RELU, Layer, check, lib
+from ._lib import ACT_LEAKY, ACT_NONE, ACT_RELU, DenseLayer, Layer, check, lib
 from .packing import CB
 
 
@@ -90,11 +90,66 @@ class QUInt8Buffer(FloatBuffer):
         return self.m_zero
 
 
+class _NarrowBuffer:
+    """A flat array of a type that only the layers of narrow types take; every other layer refuses it."""
+    dtype = torch.bfloat16
+
+    def __init__(self, num_elts=0, device="cuda", data=None):
+        if data is not None:
+            self.t = _to_device(data, self.dtype, device)
+        else:
+            self.t = torch.empty(int(num_elts), dtype=self.dtype, device=device)
+
+    size, data, ptr, swap = FloatBuffer.size, FloatBuffer.data, FloatBuffer.ptr, FloatBuffer.swap
+
+    def numpy(self):
+        return self.t.float().cpu().numpy()
+
+    @property
+    def is_cuda(self):  # asked for by _ptr of layers that know fp32 and uint8 only
+        raise ValueError(f"{type(self).__name__}: this layer takes FloatBuffer or QUInt8Buffer operands")
+
+
+class BFloat16Buffer(_NarrowBuffer):
+    """A flat array of bf16."""
+
+
+class HalfBuffer(_NarrowBuffer):
+    """A flat array of half-precision floats."""
+    dtype = torch.float16
+
+
+class Float8Buffer(_NarrowBuffer):
+    """A matrix [rows][columns] of e4m3 codes (in `t`) with an fp32 scale (in `scales`) for each block of 128 columns by `block_rows` rows:
+    1 for activations, 128 for weights.  The value of an element is its code times its block's scale."""
+    dtype = torch.float8_e4m3fn
+
+    def __init__(self, rows, columns, block_rows=1, device="cuda", data=None, scales=None):
+        if block_rows not in (1, 128):
+            raise ValueError(f"Float8Buffer: blocks of 1 or 128 rows, not {block_rows}")
+        self.rows, self.columns, self.block_rows = int(rows), int(columns), block_rows
+        n = -(-self.rows // block_rows) * -(-self.columns // 128)
+        if isinstance(data, np.ndarray):  # codes
+            data = torch.from_numpy(np.ascontiguousarray(data, np.uint8)).view(self.dtype)
+        super().__init__(self.rows * self.columns, device, data)
+        self.scales = torch.empty(n, device=device) if scales is None else _to_device(scales, torch.float32, device)
+        if self.t.numel() != self.rows * self.columns or self.scales.numel() != n:
+            raise ValueError(f"Float8Buffer: {self.t.numel()} codes and {self.scales.numel()} scales for {self.rows} x {self.columns}")
+
+    def dequantized(self):
+        """The values as an fp32 tensor [rows][columns]."""
+        s = self.scales.view(-1, -(-self.columns // 128)).repeat_interleave(self.block_rows, 0)[:self.rows]
+        return self.t.view(self.rows, self.columns).float() * s.repeat_interleave(128, 1)[:, :self.columns]
+
+
+_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
+
+
 def _to_device(data, dtype, device):
     if isinstance(data, torch.Tensor):
         return data.to(device=device, dtype=dtype).contiguous().reshape(-1)
-    np_dtype = np.float32 if dtype == torch.float32 else np.uint8
-    return torch.from_numpy(np.ascontiguousarray(data, dtype=np_dtype).reshape(-1)).to(device)
+    np_dtype = np.uint8 if dtype == torch.uint8 else np.float32
+    return torch.from_numpy(np.ascontiguousarray(data, dtype=np_dtype).reshape(-1)).to(device=device, dtype=dtype)
 
 
 _raw_stream, _device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
@@ -467,9 +522,30 @@ def Dense(output_elements, input_elements, input_buf, filter_buf, output_buf, *,
     """A fully connected layer the way the reference's models build it: Conv2D 1x1 on a 1x1
     image with FILTER_FC packing (include/small/models/DSCNNTiny.hpp:255-263).  The
     reference's own small::Dense (:2113) is an uncalled placeholder that instantiates a
-    depthwise scaling, not a matrix-vector product."""
-    Conv2D(1, 1, 1, 0, 0, 0, 0, output_elements, input_elements, 1, 1, input_buf, filter_buf,
-           output_buf, batch=batch, stream=stream)
+    depthwise scaling, not a matrix-vector product.  With Float8Buffer operands: Dense_Bias_Activation."""
+    if isinstance(filter_buf, Float8Buffer):
+        _dense_f8("Dense", output_elements, input_elements, input_buf, filter_buf, None, output_buf, 0, ACT_NONE, 0.0, batch, None, stream)
+    else:
+        Conv2D(1, 1, 1, 0, 0, 0, 0, output_elements, input_elements, 1, 1, input_buf, filter_buf,
+               output_buf, batch=batch, stream=stream)
+
+
+def Dense_Bias_Activation(output_elements, input_elements, input_buf, filter_buf, bias_buf, output_buf, *, activation=ACT_NONE,
+                          negative_slope=0.0, partial=False, batch=1, output_stride=None, stream=None):
+    """Dense with the bias / activation slots of Conv2D_Bias_Activation; bias_buf may be None.
+
+    Float8Buffer operands: activations [batch][input_elements] in blocks of 1 row, weights [output_elements][input_elements] (one row an
+    output) in blocks of 128 rows; the output is a FloatBuffer, BFloat16Buffer or HalfBuffer whose rows are output_stride elements
+    apart (packed without it), computed in fp32 and rounded once.  partial=True starts from the existing output, as the Partial* layers do.
+    input_elements is a multiple of 16, output_elements any number.  Other operands: Conv2D 1x1 on a 1x1 image, packed output."""
+    if isinstance(filter_buf, Float8Buffer):
+        _dense_f8("Dense_Bias_Activation", output_elements, input_elements, input_buf, filter_buf, bias_buf, output_buf, int(partial), activation,
+                  negative_slope, batch, output_stride, stream)
+    else:
+        if output_stride not in (None, output_elements):
+            raise ValueError("Dense_Bias_Activation: a row stride of the output needs Float8Buffer operands")
+        _conv("Dense_Bias_Activation", bool(partial), 1, 1, 1, 0, 0, 0, 0, output_elements, input_elements, 1, 1, input_buf, filter_buf,
+              output_buf, bias_buf, activation, negative_slope, batch, stream)
 
 
 # --------------------------------------------------------------------------- tensor-core fp32 conv
@@ -572,6 +648,97 @@ def Conv2D_ReLU_DepthwiseConv2D_ReLU(conv_kernel_height, conv_kernel_width, conv
     check(lib().small_b200_dwconv2d_u8(C.byref(Ld), _ptr(inter_output_buf), _ptr(dwise_filter_buf), _ptr(dw_bias),
                                        _ptr(output_buf), _stream(stream)))
     return False
+
+
+# --------------------------------------------------------------------------- narrow types
+def _narrow(name, buf, elems, what, types=None):
+    """Address of a buffer's (or a flat tensor's) elements: of an allowed type, on the current device, `elems` of them at least."""
+    t = buf.t if isinstance(buf, (FloatBuffer, _NarrowBuffer)) else buf
+    if not t.is_cuda:
+        raise _lib.SmallB200Error("buffers must live on a CUDA device (no CPU path)")
+    if t.dtype not in (types or _TYPES):
+        raise ValueError(f"{name}: {what} of type {t.dtype}")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: {what} on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: {what} is not contiguous")
+    if t.numel() < elems:
+        raise ValueError(f"{name}: {what} holds {t.numel()} elements, {elems} needed")
+    return t.data_ptr()
+
+
+def _sizes(name, *numbers):
+    for n in numbers:
+        if not 0 <= n < 1 << 31:  # a longer one would lose its upper bits on the way to the library
+            raise ValueError(f"{name}: a size of {n}")
+
+
+_F32, _F8, _TOKENS, _I32 = (torch.float32,), (torch.float8_e4m3fn,), (torch.int32, torch.int64), (torch.int32,)
+
+
+def QuantizeBlocks(num_rows, num_columns, input_buf, output_buf, *, input_stride=None, stream=None):
+    """A matrix (FloatBuffer, BFloat16Buffer or HalfBuffer; rows input_stride elements apart, packed without it) to the codes and scales
+    of a Float8Buffer: scale = largest magnitude of the block / 448 (1 for zeros), code = the exact quotient to the nearest e4m3 value, ties to
+    even.  NaN and infinities become NaN and take no part in the scale.  num_columns is a multiple of 16.  No reference counterpart."""
+    name = "QuantizeBlocks"
+    if not isinstance(output_buf, Float8Buffer):
+        raise ValueError(f"{name}: the output is a Float8Buffer")
+    if (output_buf.rows, output_buf.columns) != (num_rows, num_columns):
+        raise ValueError(f"{name}: an output of {output_buf.rows} x {output_buf.columns} for {num_rows} x {num_columns}")
+    _sizes(name, num_rows, num_columns)
+    apart = num_columns if input_stride is None else input_stride
+    x = _narrow(name, input_buf, (num_rows - 1) * apart + num_columns if num_rows > 0 else 0, "input")
+    kind = _TYPES[input_buf.t.dtype]
+    check(lib().small_b200_quantize_blocks_f8(num_rows, num_columns, output_buf.block_rows, kind, x, apart,
+                                              _narrow(name, output_buf, 0, "output", _F8), _narrow(name, output_buf.scales, 0, "scales", _F32),
+                                              _stream(stream)))
+
+
+def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, out_stride, stream):
+    if not (isinstance(inp, Float8Buffer) and isinstance(filt, Float8Buffer)):
+        raise ValueError(f"{name}: Float8Buffer operands go together")
+    if inp.block_rows != 1 or filt.block_rows != 128:
+        raise ValueError(f"{name}: activations in blocks of 1 row and weights in blocks of 128, not {inp.block_rows} and {filt.block_rows}")
+    if (filt.rows, filt.columns) != (K, C_) or inp.columns != C_ or inp.rows < rows:
+        raise ValueError(f"{name}: weights {filt.rows} x {filt.columns} and activations {inp.rows} x {inp.columns} for {rows} rows, {C_} -> {K}")
+    if not isinstance(out, (FloatBuffer, BFloat16Buffer, HalfBuffer)) or out.t.dtype not in _TYPES:
+        raise ValueError(f"{name}: the output is a FloatBuffer, BFloat16Buffer or HalfBuffer")
+    _sizes(name, rows, K, C_)
+    apart = K if out_stride is None else out_stride
+    L = _dense_layer(rows, K, C_, _TYPES[out.t.dtype], apart, accumulate, act, slope)
+    check(lib().small_b200_dense_f8(L, _narrow(name, inp, 0, "input", _F8), _narrow(name, inp.scales, 0, "input scales", _F32),
+                                    _narrow(name, filt, 0, "filter", _F8), _narrow(name, filt.scales, 0, "filter scales", _F32),
+                                    None if bias is None else _narrow(name, bias, K, "bias", _F32),
+                                    _narrow(name, out, (rows - 1) * apart + K if rows > 0 else 0, "output"), _stream(stream)))
+
+
+@functools.lru_cache(maxsize=1024)
+def _dense_layer(rows, K, C_, out_type, apart, accumulate, act, slope):
+    """The descriptor as the library takes it; nobody writes to it."""
+    return C.byref(DenseLayer(rows, K, C_, out_type, 0, 0, apart, accumulate, act, slope))
+
+
+def LogProbabilities(num_rows, num_classes, logits_buf, tokens, logprobs_buf, entropy_buf=None, top_logprobs_buf=None, top_tokens=None, *,
+                     top=0, row_stride=None, stream=None):
+    """What a model answers with, from its logits (FloatBuffer, BFloat16Buffer or HalfBuffer; rows row_stride elements apart, packed
+    without it) in one pass: the log-probability of each row's given class, the entropy of its distribution (natural units), and its `top` (at most 32)
+    best classes with their log-probabilities, in descending order, of equal logits the lowest class first.
+
+    tokens: int32 or int64 tensor [num_rows]; a negative one gives 0, one that is not below num_classes NaN.  logprobs_buf, entropy_buf
+    [num_rows] and top_logprobs_buf [num_rows][top] hold fp32, top_tokens [num_rows][top] is an int32 tensor; each may be None (and tokens
+    with logprobs_buf).  Classes at minus infinity are masked; a row with nothing else has log-probabilities of minus infinity and an entropy of 0.
+    A row with NaN or plus infinity has NaN for both.  small::SoftMax (:1778 of the reference) subtracts no maximum and knows no classes."""
+    name = "LogProbabilities"
+    _sizes(name, num_rows, num_classes, top)
+    apart = num_classes if row_stride is None else row_stride
+    x = _narrow(name, logits_buf, (num_rows - 1) * apart + num_classes if num_rows > 0 else 0, "logits")
+    given = None if tokens is None else _narrow(name, tokens, num_rows, "tokens", _TOKENS)
+    check(lib().small_b200_logprobs(
+        num_rows, num_classes, _TYPES[logits_buf.t.dtype], x, apart, 4 if tokens is None else tokens.element_size(), given,
+        None if logprobs_buf is None else _narrow(name, logprobs_buf, num_rows, "log-probabilities", _F32),
+        None if entropy_buf is None else _narrow(name, entropy_buf, num_rows, "entropy", _F32), top,
+        None if top_logprobs_buf is None else _narrow(name, top_logprobs_buf, num_rows * top, "top log-probabilities", _F32),
+        None if top_tokens is None else _narrow(name, top_tokens, num_rows * top, "top tokens", _I32), _stream(stream)))
 
 
 # --------------------------------------------------------------------------- detection head
