@@ -29,6 +29,7 @@ struct DenseArgs
     long long out_stride;
     const float *in_scales, *filt_scales, *bias;
     void *out;
+    int finish; // a bias, an activation or an old value
     int wide; // rows of the output begin on 16-byte boundaries
 };
 
@@ -301,9 +302,13 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-constexpr int MANY_N = 256, MANY_STAGE = A_BYTES + MANY_N * KB, MANY_STAGES = 4, MANY_EPI = 8, MANY_THREADS = (MANY_EPI + 2) * 32;
+// A pair of CTAs (cta_group::2) owns 256 rows by 256 outputs: each brings its 128 rows and half of the weights, 32 KB a block where a CTA by itself
+// would bring 48 KB for the same products; traffic between L2 and the SMs is what bounded that (10.4 TB/s over the device).
+constexpr int MANY_N = 256, MANY_STAGE = 2 * A_BYTES, MANY_STAGES = 6, MANY_EPI = 8, MANY_THREADS = 384;
 constexpr int MANY_SMEM = 1024 + MANY_STAGES * MANY_STAGE;
-constexpr int GROUP = 16; // tiles of rows that are walked together: their activations and the weights beside them stay in L2
+// Registers: 384 threads start with 168 each (64512 in all); the four warps that feed keep 40, the eight that fold take 232, which adds up to the same.
+constexpr int REGS_FEED = 40, REGS_FOLD = 232;
+constexpr int GROUP = 8; // tiles of rows that are walked together: their activations and the weights beside them stay in L2
 
 struct TileAt
 {
@@ -314,8 +319,23 @@ __device__ __forceinline__ TileAt tile_at(const DenseArgs &a, int t)
     const int per_group = GROUP * a.k_tiles, g = t / per_group, in = t - g * per_group;
     const int size = min(GROUP, a.r_tiles - g * GROUP);
     const int kt = in / size;
-    return {(g * GROUP + in - kt * size) * 128, kt * MANY_N};
+    return {(g * GROUP + in - kt * size) * 256, kt * MANY_N};
 }
+
+// Two sums times one scale onto two more, one instruction.
+__device__ __forceinline__ void fold2(unsigned long long &acc, uint32_t lo, uint32_t hi, unsigned long long s2)
+{
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(r), "l"(s2));
+}
+__device__ __forceinline__ void fold32(unsigned long long *acc, const uint32_t *r, unsigned long long s2)
+{
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+        fold2(acc[c], r[2 * c], r[2 * c + 1], s2);
+}
+__device__ __forceinline__ float2 pair_of(unsigned long long v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
 
 template <int TYPE>
 __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -326,69 +346,75 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
     __shared__ uint32_t tmem_s;
     uint8_t *ring = align1024(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = (int)cluster_ctarank(), pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
     const int tiles = a.k_tiles * a.r_tiles;
     if (tid == 0)
     {
         for (int s = 0; s < MANY_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], MANY_EPI); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], 2 * MANY_EPI); }
         mbar_init(&drained, 1);
         fence_barrier_init();
     }
-    if (warp == MANY_EPI + 1)
-    {
-        tmem_alloc(&tmem_s, 512);
-        tmem_relinquish();
-    }
+    if (warp == 1)
+        tmem_alloc_pair(&tmem_s, 512);
     tc_fence_before_sync();
     __syncthreads();
+    cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_s;
 
-    if (warp < MANY_EPI)
+    if (warp >= 4)
     {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_FOLD));
         // ---- thread = one row of activations and 128 outputs, a block of weights
-        const int half = warp >> 2, lane_row = (warp & 3) * 32 + lane;
+        const int half = (warp - 4) >> 2, lane_row = (warp & 3) * 32 + lane;
         const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * 128);
+        const uint32_t give_back = map_to_cta(sum_empty, 0);
         bool ok = true;
         unsigned i = 0;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+        for (int t = pair; t < tiles && ok; t += pairs)
         {
             const TileAt at = tile_at(a, t);
-            const int row = at.r0 + lane_row, k0 = at.k0 + half * 128;
+            const int row = at.r0 + rank * 128 + lane_row, k0 = at.k0 + half * 128;
             const float *sx = a.in_scales + (size_t)min(row, a.rows - 1) * a.blocks;
             const float *sw = a.filt_scales + (size_t)min(k0 / 128, (a.K - 1) / 128) * a.blocks;
-            float acc[128];
+            unsigned long long acc[64];
 #pragma unroll
-            for (int c = 0; c < 128; ++c)
-                acc[c] = 0.f;
-            float next = __ldg(sx) * __ldg(sw);
+            for (int c = 0; c < 64; ++c)
+                acc[c] = 0ull;
+            float next_x = __ldg(sx), next_w = __ldg(sw); // multiplied when they are needed: until then nothing waits for them
             for (int b = 0; b < a.blocks; ++b, ++i)
             {
                 const int buf = i & 1;
-                const float s = next;
+                const float s = next_x * next_w;
+                const unsigned long long s2 = (unsigned long long)__float_as_uint(s) << 32 | __float_as_uint(s);
                 if (b + 1 < a.blocks)
-                    next = __ldg(sx + b + 1) * __ldg(sw + b + 1);
+                {
+                    next_x = __ldg(sx + b + 1);
+                    next_w = __ldg(sw + b + 1);
+                }
                 ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[buf], (i >> 1) & 1, status, 111));
                 if (!ok)
                     break;
                 tc_fence_after_sync();
-#pragma unroll
-                for (int c0 = 0; c0 < 128; c0 += 32)
-                {
-                    uint32_t r[32];
-                    tmem_ld32(from + (uint32_t)(buf * MANY_N + c0), r);
-                    tmem_ld_wait();
-                    if (c0 == 96)
-                    {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0)
-                            mbar_arrive(&sum_empty[buf]);
-                    }
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        acc[c0 + c] = fmaf(__uint_as_float(r[c]), s, acc[c0 + c]);
-                }
+                const uint32_t src = from + (uint32_t)(buf * MANY_N);
+                uint32_t r0[32], r1[32];
+                tmem_ld32(src, r0);
+                tmem_ld_wait();
+                tmem_ld32(src + 32, r1);
+                fold32(acc, r0, s2);
+                tmem_ld_wait();
+                tmem_ld32(src + 64, r0);
+                fold32(acc + 16, r1, s2);
+                tmem_ld_wait();
+                tmem_ld32(src + 96, r1);
+                fold32(acc + 32, r0, s2);
+                tmem_ld_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive_remote_relaxed(give_back + buf * 8);
+                fold32(acc + 48, r1, s2);
             }
             if (!ok)
                 break;
@@ -403,17 +429,24 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                         break;
                     float v[VE];
 #pragma unroll
-                    for (int c = 0; c < VE; ++c)
+                    for (int c = 0; c < VE; c += 2)
                     {
-                        v[c] = acc[c0 + c];
-                        if (k0 + c0 + c < a.K)
-                        {
-                            if (a.accumulate)
-                                v[c] += load1<TYPE>(a.out, base + c0 + c);
-                            if (a.bias)
-                                v[c] += __ldg(a.bias + k0 + c0 + c);
-                            v[c] = activate(v[c], a.neg_scale);
-                        }
+                        const float2 f = pair_of(acc[(c0 + c) / 2]);
+                        v[c] = f.x;
+                        v[c + 1] = f.y;
+                    }
+                    if (a.finish)
+                    {
+#pragma unroll
+                        for (int c = 0; c < VE; ++c)
+                            if (k0 + c0 + c < a.K)
+                            {
+                                if (a.accumulate)
+                                    v[c] += load1<TYPE>(a.out, base + c0 + c);
+                                if (a.bias)
+                                    v[c] += __ldg(a.bias + k0 + c0 + c);
+                                v[c] = activate(v[c], a.neg_scale);
+                            }
                     }
                     if (a.wide && k0 + c0 + VE <= a.K)
                     {
@@ -436,62 +469,108 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             }
         }
     }
-    else if (warp == MANY_EPI)
+    else
     {
-        if (lane == 0)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEED));
+        if (warp == 0)
         {
+            // ---- this CTA's rows and its half of the weights; the first CTA's barrier counts both CTAs' bytes
             bool ok = true;
-            unsigned i = 0;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
+            unsigned i = 0, s = 0, turn = 0;
+            const uint32_t bars = map_to_cta(full, 0);
+            for (int t = pair; t < tiles && ok; t += pairs)
             {
                 const TileAt at = tile_at(a, t);
+                const int rx = at.r0 + rank * 128, rw = at.k0 + rank * 128;
                 for (int b = 0; b < a.blocks; ++b, ++i)
                 {
-                    const unsigned s = i % MANY_STAGES;
-                    if (i >= MANY_STAGES && !mbar_wait(&empty[s], (i / MANY_STAGES - 1) & 1, status, 112))
-                    {
-                        ok = false;
+                    if (turn > 0)
+                        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (turn - 1) & 1, status, 112));
+                    if (!ok)
                         break;
+                    if (elect_one())
+                    {
+                        if (rank == 0)
+                            mbar_expect_tx(&full[s], 2 * MANY_STAGE);
+                        uint8_t *dst = ring + s * MANY_STAGE;
+                        tma_load_2d_pair(dst, &map_x, b * KB, rx, bars + s * 8);
+                        tma_load_2d_pair(dst + A_BYTES, &map_w, b * KB, rw, bars + s * 8);
                     }
-                    mbar_expect_tx(&full[s], MANY_STAGE);
-                    tma_load_2d(ring + s * MANY_STAGE, &map_x, b * KB, at.r0, &full[s]);
-                    tma_load_2d(ring + s * MANY_STAGE + A_BYTES, &map_w, b * KB, at.k0, &full[s]);
+                    __syncwarp();
+                    if (++s == MANY_STAGES)
+                    {
+                        s = 0;
+                        ++turn;
+                    }
                 }
             }
-            for (unsigned j = i > MANY_STAGES ? i - MANY_STAGES : 0; j < i && !ok; ++j) // its own copies in flight
-                mbar_wait(&full[j % MANY_STAGES], (j / MANY_STAGES) & 1, status, 113);
-        }
-    }
-    else if (lane == 0)
-    {
-        const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 128, MANY_N);
-        bool ok = true;
-        unsigned i = 0;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x)
-            for (int b = 0; b < a.blocks; ++b, ++i)
+            if (!ok) // copies in flight: the first CTA sees both CTAs' arrive; a millisecond is far longer than any takes
             {
-                const unsigned s = i % MANY_STAGES, buf = i & 1;
-                ok = mbar_wait(&full[s], (i / MANY_STAGES) & 1, status, 114) &&
-                     (i < 2 || mbar_wait(&sum_empty[buf], ((i >> 1) - 1) & 1, status, 115));
-                if (!ok)
-                    break;
-                tc_fence_after_sync();
-                const uint32_t sa = smem_u32(ring + s * MANY_STAGE);
-                mma_block(tmem + buf * MANY_N, sa, sa + A_BYTES, idesc);
-                tc_commit(&empty[s]);
-                tc_commit(&sum_full[buf]);
+                for (unsigned j = i > MANY_STAGES ? i - MANY_STAGES : 0; j < i && rank == 0; ++j)
+                    mbar_wait(&full[j % MANY_STAGES], (j / MANY_STAGES) & 1, status, 113);
+                for (int n = 0; n < 1000; ++n)
+                    __nanosleep(1000);
             }
-        if (!ok)
+        }
+        else if (warp == 1 && rank == 0)
         {
-            tc_commit(&drained);
-            mbar_wait(&drained, 0, status, 116);
+            // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.  What the next block
+            // waits for is asked for between this block's MMAs: a wait costs 100 cycles even where it has nothing to wait for.
+            const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 256, MANY_N);
+            const uint64_t first_a = make_smem_desc(smem_u32(ring), 16, 1024, 2), first_b = make_smem_desc(smem_u32(ring) + A_BYTES, 16, 1024, 2);
+            const int mine = (tiles - pair + pairs - 1) / pairs;
+            const unsigned total = (unsigned)mine * (unsigned)a.blocks;
+            unsigned s = 0, turn = 0; // stage and how often all stages have been round
+            bool ok = total == 0 || mbar_wait(&full[0], 0, status, 114);
+            for (unsigned i = 0; i < total && ok; ++i)
+            {
+                const unsigned buf = i & 1;
+                const unsigned s1 = s + 1 == MANY_STAGES ? 0 : s + 1, turn1 = s + 1 == MANY_STAGES ? turn + 1 : turn;
+                tc_fence_after_sync();
+                const uint32_t d = tmem + buf * MANY_N;
+                const uint64_t da = first_a + s * (MANY_STAGE / 16), db = first_b + s * (MANY_STAGE / 16);
+                const bool leader = elect_one();
+                if (leader)
+                {
+                    tc_mma_f8_pair(d, da, db, idesc, 0u);
+                    tc_mma_f8_pair(d, da + 2, db + 2, idesc, 1u);
+                    tc_mma_f8_pair(d, da + 4, db + 4, idesc, 1u);
+                    tc_mma_f8_pair(d, da + 6, db + 6, idesc, 1u);
+                    tc_commit_pair(&empty[s]);
+                    tc_commit_pair(&sum_full[buf]);
+                }
+                __syncwarp();
+                if (i + 1 < total)
+                {
+                    // block i + 1 uses the other buffer, for the (i + 1) / 2 th time; before its first use there is nothing to wait for, which is the
+                    // parity of the phase before the first
+                    const uint32_t p = (((i + 1) >> 1) + 1) & 1;
+                    for (uint32_t n = 0; !mbar_test_both(&full[s1], turn1 & 1, &sum_empty[buf ^ 1], p); ++n)
+                        if (n >= 256) // long enough for every turn but the first ones: now the wait that gives up
+                        {
+                            ok = mbar_wait(&full[s1], turn1 & 1, status, 114) && mbar_wait(&sum_empty[buf ^ 1], p, status, 115);
+                            break;
+                        }
+                    ok = __all_sync(0xffffffffu, ok);
+                }
+                s = s1;
+                turn = turn1;
+            }
+            if (!ok)
+            {
+                if (elect_one())
+                    tc_commit_pair(&drained);
+                __syncwarp();
+                mbar_wait(&drained, 0, status, 116);
+            }
         }
     }
     __syncwarp();
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == MANY_EPI + 1)
-        tmem_dealloc(tmem, 512);
+    cluster_sync_all(); // neither CTA goes while the other may still write to it
+    if (warp == 1)
+        tmem_dealloc_pair(tmem, 512);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -557,9 +636,9 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
         }
     }
     a.k_tiles = (D->K + MANY_N - 1) / MANY_N;
-    a.r_tiles = (D->rows + 127) / 128;
+    a.r_tiles = (D->rows + 255) / 256;
     a.split = 1;
-    if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, MANY_N))
+    if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, 128))
         return rc;
     if (int rc = map_rows(&map_x, in, D->rows, D->C, in_stride, 128))
         return rc;
@@ -569,10 +648,24 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
     if (configured.needed(&dev))
     {
         SB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MANY_SMEM));
+        cudaFuncAttributes fa;
+        SB_CUDA(cudaFuncGetAttributes(&fa, kern));
+        if (fa.numRegs * MANY_THREADS < 128 * REGS_FEED + 256 * REGS_FOLD) // the split would wait for registers that the launch does not have
+            return fail(SMALL_B200_CUDA_ERROR, "dense_f8_many_kernel was built with too few registers");
         configured.mark(dev);
     }
-    const int tiles = a.k_tiles * a.r_tiles;
-    kern<<<std::min(tiles, num_sms()), MANY_THREADS, MANY_SMEM, st>>>(map_x, map_w, a, status);
+    const int pairs = std::min(a.k_tiles * a.r_tiles, num_sms() / 2);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * pairs));
+    cfg.blockDim = dim3(MANY_THREADS);
+    cfg.dynamicSmemBytes = MANY_SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SB_CUDA(cudaLaunchKernelEx(&cfg, kern, map_x, map_w, a, status));
     return launched("dense_f8_many_kernel");
 }
 } // namespace
@@ -610,6 +703,7 @@ extern "C" int small_b200_dense_f8(const small_b200_dense *D, const void *in, co
     a.rows = D->rows; a.K = D->K; a.blocks = (D->C + KB - 1) / KB;
     a.accumulate = D->accumulate; a.neg_scale = D->act == SMALL_B200_ACT_RELU ? 0.f : D->act == SMALL_B200_ACT_LEAKY ? D->slope : 1.f;
     a.out_stride = out_stride; a.in_scales = in_scales; a.filt_scales = filt_scales; a.bias = bias; a.out = out;
+    a.finish = bias || D->accumulate || D->act != SMALL_B200_ACT_NONE;
     a.wide = !off(out, 16) && out_stride * size % 16 == 0;
     cudaStream_t st = as_stream(stream);
     switch (D->out_type)

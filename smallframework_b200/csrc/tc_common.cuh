@@ -96,6 +96,20 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
                  : "memory");
     return ok != 0;
 }
+// Have both phases completed?  The two questions are under way together: a loop for each takes 80 to 160 cycles even where there is nothing to
+// wait for.
+__device__ __forceinline__ bool mbar_test_both(uint64_t *a, uint32_t parity_a, uint64_t *b, uint32_t parity_b)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p, q;\n\t"
+                 "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "mbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+                 "and.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(smem_u32(a)), "r"(parity_a), "r"(smem_u32(b)), "r"(parity_b)
+                 : "memory");
+    return ok != 0;
+}
 // Bounded wait: gives up after `limit` polls (each poll itself blocks for a
 // hardware-defined short time), records the failure and returns false.
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, int *status, int code,
@@ -134,6 +148,12 @@ __device__ __forceinline__ uint32_t map_to_cta(const void *p, uint32_t rank)
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr)
 {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The same where nothing but the arrival itself has to be seen (tensor memory that has been read, after its wait): a release waits for every
+// memory operation of the thread, 1300 cycles where loads from global memory are under way.
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr)
 {
@@ -274,6 +294,38 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// ---- pairs of CTAs (a cluster of two) that share one MMA: M = 256, each CTA has 128 rows of A, half of B's rows and its 128 rows of D
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *dst_smem, uint32_t ncols)
+{
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols)
+{
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tc_mma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// Arrive on the barrier at this offset in both CTAs once every MMA issued so far by this thread has completed.
+__device__ __forceinline__ void tc_commit_pair(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+// Into this CTA's shared memory, counted by a barrier in either CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, int c0, int c1, uint32_t cluster_bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(cluster_bar)
                  : "memory");
 }
 // Half-precision operands with D = A * B + D * 2^-DOWN: what the accumulator holds is brought to another scale on the way.
