@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
 // A pair of CTAs (cta_group::2) owns 256 rows by 256 outputs: each brings its 128 rows and half of the weights, 32 KB a block where a CTA by itself
 // would bring 48 KB for the same products; traffic between L2 and the SMs is what bounded that (10.4 TB/s over the device).
 constexpr int MANY_N = 256, MANY_STAGE = 2 * A_BYTES, MANY_STAGES = 6, MANY_EPI = 8, MANY_THREADS = 384;
+static_assert(MANY_STAGES % 2 == 0, "a buffer's blocks keep to every other stage");
 constexpr int MANY_SMEM = 1024 + MANY_STAGES * MANY_STAGE;
 // Registers: 384 threads start with 168 each (64512 in all); the four warps that feed keep 40, the eight that fold take 232, which adds up to the same.
 constexpr int REGS_FEED = 40, REGS_FOLD = 232;
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                                                                           const DenseArgs a, int *status)
 {
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[MANY_STAGES], empty[MANY_STAGES], sum_full[2], sum_empty[2], drained;
+    __shared__ uint64_t full[MANY_STAGES], empty[MANY_STAGES], sum_full[2], sum_empty[2], drained[2];
     __shared__ uint32_t tmem_s;
     uint8_t *ring = align1024(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -351,11 +352,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
     if (tid == 0)
     {
         for (int s = 0; s < MANY_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], 2 * MANY_EPI); }
-        mbar_init(&drained, 1);
+        for (int s = 0; s < 2; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], 2 * MANY_EPI); mbar_init(&drained[s], 1); }
         fence_barrier_init();
     }
-    if (warp == 1)
+    if (warp == 3)
         tmem_alloc_pair(&tmem_s, 512);
     tc_fence_before_sync();
     __syncthreads();
@@ -382,24 +382,27 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
 #pragma unroll
             for (int c = 0; c < 64; ++c)
                 acc[c] = 0ull;
+            // Software pipeline over the blocks: while 32 columns are folded the next 32 are on their way, across blocks too, and the next block's
+            // barrier is asked one step before its answer is needed.
             float next_x = __ldg(sx), next_w = __ldg(sw); // multiplied when they are needed: until then nothing waits for them
+            uint32_t r0[32], r1[32];
+            ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[i & 1], (i >> 1) & 1, status, 111));
+            if (!ok)
+                break;
+            tc_fence_after_sync();
+            tmem_ld32(from + (uint32_t)((i & 1) * MANY_N), r0);
             for (int b = 0; b < a.blocks; ++b, ++i)
             {
                 const int buf = i & 1;
+                const uint32_t src = from + (uint32_t)(buf * MANY_N);
                 const float s = next_x * next_w;
                 const unsigned long long s2 = (unsigned long long)__float_as_uint(s) << 32 | __float_as_uint(s);
-                if (b + 1 < a.blocks)
+                const bool more = b + 1 < a.blocks;
+                if (more)
                 {
                     next_x = __ldg(sx + b + 1);
                     next_w = __ldg(sw + b + 1);
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[buf], (i >> 1) & 1, status, 111));
-                if (!ok)
-                    break;
-                tc_fence_after_sync();
-                const uint32_t src = from + (uint32_t)(buf * MANY_N);
-                uint32_t r0[32], r1[32];
-                tmem_ld32(src, r0);
                 tmem_ld_wait();
                 tmem_ld32(src + 32, r1);
                 fold32(acc, r0, s2);
@@ -408,12 +411,24 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                 fold32(acc + 16, r1, s2);
                 tmem_ld_wait();
                 tmem_ld32(src + 96, r1);
+                const bool ready = more && mbar_test(&sum_full[buf ^ 1], ((i + 1) >> 1) & 1);
                 fold32(acc + 32, r0, s2);
                 tmem_ld_wait();
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive_remote_relaxed(give_back + buf * 8);
+                if (more)
+                {
+                    if (!__all_sync(0xffffffffu, ready))
+                    {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[buf ^ 1], ((i + 1) >> 1) & 1, status, 111));
+                        if (!ok)
+                            break;
+                    }
+                    tc_fence_after_sync();
+                    tmem_ld32(from + (uint32_t)((buf ^ 1) * MANY_N), r0);
+                }
                 fold32(acc + 48, r1, s2);
             }
             if (!ok)
@@ -512,56 +527,52 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                     __nanosleep(1000);
             }
         }
-        else if (warp == 1 && rank == 0)
+        else if ((warp == 1 || warp == 2) && rank == 0)
         {
-            // The whole warp walks the loop, so that addresses and descriptors stay in uniform registers; one lane issues.  What the next block
-            // waits for is asked for between this block's MMAs: a wait costs 100 cycles even where it has nothing to wait for.
+            // One warp for each buffer of sums, every other block its own: what a warp does around its MMAs (500 cycles a block, most of it waiting for
+            // answers) then passes behind the other's.  The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
             const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 256, MANY_N);
             const uint64_t first_a = make_smem_desc(smem_u32(ring), 16, 1024, 2), first_b = make_smem_desc(smem_u32(ring) + A_BYTES, 16, 1024, 2);
-            const int mine = (tiles - pair + pairs - 1) / pairs;
-            const unsigned total = (unsigned)mine * (unsigned)a.blocks;
-            unsigned s = 0, turn = 0; // stage and how often all stages have been round
-            bool ok = total == 0 || mbar_wait(&full[0], 0, status, 114);
-            for (unsigned i = 0; i < total && ok; ++i)
+            const unsigned buf = warp - 1, total = (unsigned)((tiles - pair + pairs - 1) / pairs) * (unsigned)a.blocks;
+            const uint32_t d = tmem + buf * MANY_N;
+            unsigned s = buf, turn = 0, use = 1; // stage, parity of its phase, parity of the phase before the buffer's next use
+            bool ok = true;
+            for (unsigned i = buf; i < total; i += 2)
             {
-                const unsigned buf = i & 1;
-                const unsigned s1 = s + 1 == MANY_STAGES ? 0 : s + 1, turn1 = s + 1 == MANY_STAGES ? turn + 1 : turn;
+                for (uint32_t n = 0; !mbar_test_both(&full[s], turn, &sum_empty[buf], use); ++n)
+                    if (n >= 256) // long enough for every turn but the first ones: now the wait that gives up
+                    {
+                        ok = mbar_wait(&full[s], turn, status, 114) && mbar_wait(&sum_empty[buf], use, status, 115);
+                        break;
+                    }
+                if (!__all_sync(0xffffffffu, ok))
+                    break;
                 tc_fence_after_sync();
-                const uint32_t d = tmem + buf * MANY_N;
-                const uint64_t da = first_a + s * (MANY_STAGE / 16), db = first_b + s * (MANY_STAGE / 16);
-                const bool leader = elect_one();
-                if (leader)
+                if (elect_one())
                 {
+                    const uint64_t da = first_a + s * (MANY_STAGE / 16), db = first_b + s * (MANY_STAGE / 16);
                     tc_mma_f8_pair(d, da, db, idesc, 0u);
                     tc_mma_f8_pair(d, da + 2, db + 2, idesc, 1u);
                     tc_mma_f8_pair(d, da + 4, db + 4, idesc, 1u);
                     tc_mma_f8_pair(d, da + 6, db + 6, idesc, 1u);
-                    tc_commit_pair(&empty[s]);
                     tc_commit_pair(&sum_full[buf]);
+                    tc_commit_pair(&empty[s]);
                 }
                 __syncwarp();
-                if (i + 1 < total)
+                use ^= 1;
+                s += 2;
+                if (s >= MANY_STAGES)
                 {
-                    // block i + 1 uses the other buffer, for the (i + 1) / 2 th time; before its first use there is nothing to wait for, which is the
-                    // parity of the phase before the first
-                    const uint32_t p = (((i + 1) >> 1) + 1) & 1;
-                    for (uint32_t n = 0; !mbar_test_both(&full[s1], turn1 & 1, &sum_empty[buf ^ 1], p); ++n)
-                        if (n >= 256) // long enough for every turn but the first ones: now the wait that gives up
-                        {
-                            ok = mbar_wait(&full[s1], turn1 & 1, status, 114) && mbar_wait(&sum_empty[buf ^ 1], p, status, 115);
-                            break;
-                        }
-                    ok = __all_sync(0xffffffffu, ok);
+                    s -= MANY_STAGES;
+                    turn ^= 1;
                 }
-                s = s1;
-                turn = turn1;
             }
-            if (!ok)
+            if (!__all_sync(0xffffffffu, ok))
             {
                 if (elect_one())
-                    tc_commit_pair(&drained);
+                    tc_commit_pair(&drained[buf]);
                 __syncwarp();
-                mbar_wait(&drained, 0, status, 116);
+                mbar_wait(&drained[buf], 0, status, 116);
             }
         }
     }
@@ -569,7 +580,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync_all(); // neither CTA goes while the other may still write to it
-    if (warp == 1)
+    if (warp == 3)
         tmem_dealloc_pair(tmem, 512);
 }
 
