@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
 // would bring 48 KB for the same products; traffic between L2 and the SMs is what bounded that (10.4 TB/s over the device).
 constexpr int MANY_N = 256, MANY_STAGE = 2 * A_BYTES, MANY_STAGES = 6, MANY_EPI = 8, MANY_THREADS = 384;
 static_assert(MANY_STAGES % 2 == 0, "a buffer's blocks keep to every other stage");
-constexpr int MANY_SMEM = 1024 + MANY_STAGES * MANY_STAGE;
+constexpr int STAGE_OUT = 32 * 128; // a warp's way out
+constexpr int MANY_SMEM = 1024 + MANY_STAGES * MANY_STAGE + MANY_EPI * STAGE_OUT;
 // Registers: 384 threads start with 168 each (64512 in all); the four warps that feed keep 40, the eight that fold take 232, which adds up to the same.
 constexpr int REGS_FEED = 40, REGS_FOLD = 232;
 constexpr int GROUP = 8; // tiles of rows that are walked together: their activations and the weights beside them stay in L2
@@ -433,20 +434,23 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             }
             if (!ok)
                 break;
-            if (row < a.rows)
-            {
-                const long long base = (long long)row * a.out_stride + k0;
-                constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE;
+            // Out through shared memory: a thread's 128 bytes of a row go in, whole lines of four rows come out.  Straight from the registers every
+            // 16-byte store of a warp touches 32 lines, and a tile took 5000 cycles.
+            constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, WIDE = 8 * VE;
+            uint8_t *stage = ring + MANY_STAGES * MANY_STAGE + (warp - 4) * STAGE_OUT;
 #pragma unroll
-                for (int c0 = 0; c0 < 128; c0 += VE)
+            for (int c0 = 0; c0 < 128; c0 += WIDE)
+            {
+                if (k0 + c0 >= a.K)
+                    break;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
                 {
-                    if (k0 + c0 >= a.K)
-                        break;
                     float v[VE];
 #pragma unroll
                     for (int c = 0; c < VE; c += 2)
                     {
-                        const float2 f = pair_of(acc[(c0 + c) / 2]);
+                        const float2 f = pair_of(acc[(c0 + j * VE + c) / 2]);
                         v[c] = f.x;
                         v[c + 1] = f.y;
                     }
@@ -454,33 +458,50 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                     {
 #pragma unroll
                         for (int c = 0; c < VE; ++c)
-                            if (k0 + c0 + c < a.K)
-                            {
-                                if (a.accumulate)
-                                    v[c] += load1<TYPE>(a.out, base + c0 + c);
-                                if (a.bias)
-                                    v[c] += __ldg(a.bias + k0 + c0 + c);
-                                v[c] = activate(v[c], a.neg_scale);
-                            }
+                        {
+                            const int k = k0 + c0 + j * VE + c;
+                            if (a.accumulate && k < a.K && row < a.rows)
+                                v[c] += load1<TYPE>(a.out, (long long)row * a.out_stride + k);
+                            if (a.bias && k < a.K)
+                                v[c] += __ldg(a.bias + k);
+                            v[c] = activate(v[c], a.neg_scale);
+                        }
                     }
-                    if (a.wide && k0 + c0 + VE <= a.K)
-                    {
-                        uint4 w;
-                        if (TYPE == SMALL_B200_TYPE_F32)
-                            w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-                        else
-                            w = make_uint4(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]), pack2<TYPE>(v[VE - 4], v[VE - 3]),
-                                           pack2<TYPE>(v[VE - 2], v[VE - 1]));
-                        *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + (base + c0) * SIZE) = w;
-                    }
+                    uint4 w;
+                    if (TYPE == SMALL_B200_TYPE_F32)
+                        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                    else
+                        w = make_uint4(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]), pack2<TYPE>(v[VE - 4], v[VE - 3]),
+                                       pack2<TYPE>(v[VE - 2], v[VE - 1]));
+                    *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = w; // no two lanes of eight share banks
+                }
+                __syncwarp();
+                const int j = lane & 7, k = k0 + c0 + j * VE;
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+                {
+                    const int r = n * 4 + (lane >> 3), to = at.r0 + rank * 128 + (warp & 3) * 32 + r;
+                    const uint4 w = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((j ^ (r & 7)) << 4));
+                    if (to >= a.rows || k >= a.K)
+                        continue;
+                    char *dst = static_cast<char *>(a.out) + ((long long)to * a.out_stride + k) * SIZE;
+                    if (a.wide && k + VE <= a.K)
+                        *reinterpret_cast<uint4 *>(dst) = w;
                     else
                     {
+                        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                         for (int c = 0; c < VE; ++c)
-                            if (k0 + c0 + c < a.K)
-                                store1<TYPE>(a.out, base + c0 + c, v[c]);
+                            if (k + c < a.K)
+                            {
+                                if (SIZE == 4)
+                                    reinterpret_cast<uint32_t *>(dst)[c] = word[c / (VE / 4)];
+                                else
+                                    reinterpret_cast<uint16_t *>(dst)[c] = (uint16_t)(word[c / (VE / 4)] >> (16 * (c & 1)));
+                            }
                     }
                 }
+                __syncwarp();
             }
         }
     }
