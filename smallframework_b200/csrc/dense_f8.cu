@@ -6,7 +6,7 @@
 // fp32 registers, times the two scales.  Tensor memory holds several blocks' sums, so that the next MMAs run meanwhile.
 //
 // Two kernels:
-//   few    weights are the 128 lanes, 16 to 128 rows of activations the columns.  The weights' bytes bound it: they come once, by TMA, into all SMs,
+//   few    weights are the 128 lanes, 16, 32 or 64 rows of activations the columns.  The weights' bytes bound it: they come once, by TMA, into all SMs,
 //          the reduction cut among the CTAs of a cluster where output tiles are few; the parts are added over distributed shared memory, in order.
 //   many   128 rows of activations are the lanes, 256 outputs the columns.  The tensor cores bound it; one CTA an SM takes tile after tile.
 #include <algorithm>
@@ -47,13 +47,14 @@ __device__ __forceinline__ void store1(void *p, long long at, float v)
         static_cast<__half *>(p)[at] = __float2half_rn(v);
 }
 
-// The four MMAs of one block: both operands K-major with 128-byte swizzle, eight rows 1024 bytes apart.
-__device__ __forceinline__ void mma_block(uint32_t d, uint32_t sa, uint32_t sb_, uint32_t idesc)
+// Two sums times their scales onto two more, one instruction.
+__device__ __forceinline__ void fold2(unsigned long long &acc, uint32_t lo, uint32_t hi, unsigned long long s2)
 {
-#pragma unroll
-    for (int k = 0; k < KB / 32; ++k)
-        tc_mma_f8(d, make_smem_desc(sa + 32 * k, 16, 1024, 2), make_smem_desc(sb_ + 32 * k, 16, 1024, 2), idesc, k > 0 ? 1u : 0u);
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(r), "l"(s2));
 }
+__device__ __forceinline__ float2 pair_of(unsigned long long v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
 
 __device__ __forceinline__ uint8_t *align1024(uint8_t *p) { return p + ((1024u - (smem_u32(p) & 1023u)) & 1023u); }
 
@@ -61,13 +62,50 @@ __device__ __forceinline__ uint8_t *align1024(uint8_t *p) { return p + ((1024u -
 template <int BN>
 struct Few
 {
-    static constexpr int STAGE = A_BYTES + BN * KB, STAGES = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
-    static constexpr int BUFS = BN == 128 ? 2 : 4, COLS = BUFS * BN;
+    // two CTAs an SM: 113 KB of shared memory and 256 columns of tensor memory each
+    static constexpr int STAGE = A_BYTES + BN * KB, STAGES = BN == 16 ? 5 : BN == 32 ? 4 : 3;
+    static constexpr int BUFS = 4, COLS = BUFS * BN;
     static constexpr int CHUNK = 8; // blocks whose scales are brought at a time
-    static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * CHUNK * BN * 4;
-    static_assert(STAGES * STAGE >= BN * 128 * 4, "the ring holds the sums that a cluster adds");
+    static constexpr int SCALES = 2 * CHUNK * BN * 4, INBOX = BN * 128 * 4;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES + INBOX;
+    static_assert(2 * (SMEM + 2048) <= 228 * 1024 && 2 * COLS <= 512, "two CTAs an SM");
 };
 constexpr int FEW_THREADS = 7 * 32;
+
+// Four consecutive outputs of a row.
+template <int TYPE>
+__device__ __forceinline__ void finish4(const DenseArgs &a, int row, int k, float4 v4)
+{
+    float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    const long long at = (long long)row * a.out_stride + k;
+    if (a.finish)
+    {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (k + c < a.K)
+            {
+                if (a.accumulate)
+                    v[c] += load1<TYPE>(a.out, at + c);
+                if (a.bias)
+                    v[c] += __ldg(a.bias + k + c);
+                v[c] = activate(v[c], a.neg_scale);
+            }
+    }
+    if (a.wide && k + 4 <= a.K)
+    {
+        if (TYPE == SMALL_B200_TYPE_F32)
+            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
+    }
+    else
+    {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (k + c < a.K)
+                store1<TYPE>(a.out, at + c, v[c]);
+    }
+}
 
 template <int BN, int TYPE>
 __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
@@ -75,56 +113,95 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
 {
     using G = Few<BN>;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[G::STAGES], empty[G::STAGES], sum_full[G::BUFS], sum_empty[G::BUFS], sc_full[2], sc_empty[2], drained;
+    __shared__ uint64_t full[G::STAGES], empty[G::STAGES], sum_full[G::BUFS], sum_empty[G::BUFS], sc_full[2], sc_empty[2], drained, delivered;
     __shared__ uint32_t tmem_s;
     uint8_t *ring = align1024(raw);
     float *scales = reinterpret_cast<float *>(ring + G::STAGES * G::STAGE); // [2][CHUNK][BN]
+    // What the cluster's CTAs have of this CTA's share of the rows, in pairs of rows: [split][rows / split / 2][128 outputs][2]
+    unsigned long long *inbox = reinterpret_cast<unsigned long long *>(ring + G::STAGES * G::STAGE + G::SCALES);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = (int)(blockIdx.x % a.split), tile = (int)(blockIdx.x / a.split);
     const int kt = tile % a.k_tiles, r0 = tile / a.k_tiles * BN;
     const int share = (a.blocks + a.split - 1) / a.split;
     const int b0 = rank * share, n = max(0, min(a.blocks, b0 + share) - b0);
+    auto load = [&](int i, int s) {
+        mbar_expect_tx(&full[s], G::STAGE);
+        tma_load_2d(ring + s * G::STAGE, &map_w, (b0 + i) * KB, kt * 128, &full[s]);
+        tma_load_2d(ring + s * G::STAGE + A_BYTES, &map_x, (b0 + i) * KB, r0, &full[s]);
+    };
 
-    if (tid == 0)
+    if (warp == 4)
     {
-        for (int s = 0; s < G::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        // the first stages are on their way before anything else is set up
+        if (elect_one())
+        {
+            for (int s = 0; s < G::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+            fence_barrier_init();
+            for (int i = 0; i < G::STAGES && i < n; ++i)
+                load(i, i);
+        }
+        __syncwarp();
+    }
+    else if (warp == 5)
+    {
+        tmem_alloc(&tmem_s, G::COLS);
+        tmem_relinquish();
+    }
+    else if (tid == 0)
+    {
         for (int s = 0; s < G::BUFS; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], 4); }
         for (int s = 0; s < 2; ++s) { mbar_init(&sc_full[s], 1); mbar_init(&sc_empty[s], 4); }
         mbar_init(&drained, 1);
+        mbar_init(&delivered, 1);
         fence_barrier_init();
+        mbar_expect_tx(&delivered, G::INBOX);
     }
-    if (warp == 5)
-    {
-        tmem_alloc(&tmem_s, G::COLS < 32 ? 32 : G::COLS);
-        tmem_relinquish();
-    }
+    // ---- scales: the product of a row's and the weights' scale, by block and row; the first ones are asked for here
+    constexpr int ROWS = (BN + 31) / 32;
+    float sv[ROWS][G::CHUNK];
+    auto ask = [&](int c) {
+        const float *sw = a.filt_scales + (size_t)kt * a.blocks + b0;
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q)
+        {
+            const int col = q * 32 + lane, row = r0 + col;
+            const float *sx = a.in_scales + (size_t)row * a.blocks + b0;
+#pragma unroll
+            for (int j = 0; j < G::CHUNK; ++j)
+            {
+                const int b = c * G::CHUNK + j;
+                sv[q][j] = col < BN && row < a.rows && b < n ? __ldg(sx + b) * __ldg(sw + b) : 0.f;
+            }
+        }
+    };
+    if (warp == 6)
+        ask(0);
     tc_fence_before_sync();
     __syncthreads();
+    cluster_arrive_release(); // this CTA's inbox can be written to
     tc_fence_after_sync();
     const uint32_t tmem = tmem_s;
-    float acc[BN];
+    unsigned long long acc[BN / 2]; // of the folding warps
 
     if (warp < 4)
     {
         // ---- thread = one output channel: folds every block's sums into registers
 #pragma unroll
-        for (int c = 0; c < BN; ++c)
-            acc[c] = 0.f;
+        for (int c = 0; c < BN / 2; ++c)
+            acc[c] = 0ull;
         bool ok = true;
-        for (int i = 0; i < n && ok; ++i)
+        for (int i = 0; i < n; ++i)
         {
             const int buf = i % G::BUFS, chunk = i / G::CHUNK;
             if (i % G::CHUNK == 0)
                 ok = mbar_wait(&sc_full[chunk & 1], (chunk >> 1) & 1, status, 101);
             ok = ok && mbar_wait(&sum_full[buf], (i / G::BUFS) & 1, status, 102);
-            if (!__all_sync(0xffffffffu, ok))
-            {
-                ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok)
                 break;
-            }
             tc_fence_after_sync();
             const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(buf * BN);
-            const float4 *s4 = reinterpret_cast<const float4 *>(scales + ((chunk & 1) * G::CHUNK + i % G::CHUNK) * BN);
+            const ulonglong2 *s4 = reinterpret_cast<const ulonglong2 *>(scales + ((chunk & 1) * G::CHUNK + i % G::CHUNK) * BN);
             constexpr int STEP = BN < 32 ? 16 : 32;
 #pragma unroll
             for (int c0 = 0; c0 < BN; c0 += STEP)
@@ -145,11 +222,9 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
 #pragma unroll
                 for (int c = 0; c < STEP; c += 4)
                 {
-                    const float4 s = s4[(c0 + c) / 4];
-                    acc[c0 + c] = fmaf(__uint_as_float(r[c]), s.x, acc[c0 + c]);
-                    acc[c0 + c + 1] = fmaf(__uint_as_float(r[c + 1]), s.y, acc[c0 + c + 1]);
-                    acc[c0 + c + 2] = fmaf(__uint_as_float(r[c + 2]), s.z, acc[c0 + c + 2]);
-                    acc[c0 + c + 3] = fmaf(__uint_as_float(r[c + 3]), s.w, acc[c0 + c + 3]);
+                    const ulonglong2 s = s4[(c0 + c) / 4];
+                    fold2(acc[(c0 + c) / 2], r[c], r[c + 1], s.x);
+                    fold2(acc[(c0 + c) / 2 + 1], r[c + 2], r[c + 3], s.y);
                 }
             }
             if (i % G::CHUNK == G::CHUNK - 1)
@@ -162,74 +237,77 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
     }
     else if (warp == 4)
     {
-        if (lane == 0)
+        bool ok = true;
+        int i = min(n, G::STAGES), s = i % G::STAGES;
+        uint32_t turn = 0;
+        for (; i < n; ++i)
         {
-            bool ok = true;
-            int i = 0;
-            for (; i < n; ++i)
+            ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], turn, status, 103));
+            if (!ok)
+                break;
+            if (elect_one())
+                load(i, s);
+            __syncwarp();
+            if (++s == G::STAGES)
             {
-                const int s = i % G::STAGES;
-                if (i >= G::STAGES && !mbar_wait(&empty[s], (i / G::STAGES - 1) & 1, status, 103))
-                {
-                    ok = false;
-                    break;
-                }
-                mbar_expect_tx(&full[s], G::STAGE);
-                tma_load_2d(ring + s * G::STAGE, &map_w, (b0 + i) * KB, kt * 128, &full[s]);
-                tma_load_2d(ring + s * G::STAGE + A_BYTES, &map_x, (b0 + i) * KB, r0, &full[s]);
+                s = 0;
+                turn ^= 1;
             }
-            for (int j = max(0, i - G::STAGES); j < i && !ok; ++j) // its own copies in flight
-                mbar_wait(&full[j % G::STAGES], (j / G::STAGES) & 1, status, 104);
         }
+        for (int j = max(0, i - G::STAGES); j < i && !ok; ++j) // its own copies in flight
+            mbar_wait(&full[j % G::STAGES], (j / G::STAGES) & 1, status, 104);
     }
     else if (warp == 5)
     {
-        if (lane == 0)
+        const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 128, BN);
+        const uint64_t first_a = make_smem_desc(smem_u32(ring), 16, 1024, 2), first_b = make_smem_desc(smem_u32(ring) + A_BYTES, 16, 1024, 2);
+        bool ok = true;
+        int s = 0;
+        uint32_t turn = 0;
+        for (int i = 0; i < n; ++i)
         {
-            const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 128, BN);
-            bool ok = true;
-            for (int i = 0; i < n && ok; ++i)
-            {
-                const int s = i % G::STAGES, buf = i % G::BUFS;
-                ok = mbar_wait(&full[s], (i / G::STAGES) & 1, status, 105) &&
-                     (i < G::BUFS || mbar_wait(&sum_empty[buf], (i / G::BUFS - 1) & 1, status, 106));
-                if (!ok)
-                    break;
-                tc_fence_after_sync();
-                const uint32_t sa = smem_u32(ring + s * G::STAGE);
-                mma_block(tmem + (uint32_t)(buf * BN), sa, sa + A_BYTES, idesc);
-                tc_commit(&empty[s]);
-                tc_commit(&sum_full[buf]);
-            }
+            const int buf = i % G::BUFS;
+            const uint32_t use = ((i / G::BUFS) & 1) ^ 1; // before a buffer's first use the phase before the first counts as complete
+            if (!mbar_test_both(&full[s], turn, &sum_empty[buf], use))
+                ok = mbar_wait(&full[s], turn, status, 105) && mbar_wait(&sum_empty[buf], use, status, 106);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok)
+                break;
+            tc_fence_after_sync();
+            if (elect_one())
             {
-                tc_commit(&drained);
-                mbar_wait(&drained, 0, status, 107);
+                const uint32_t d = tmem + (uint32_t)(buf * BN);
+                const uint64_t da = first_a + s * (G::STAGE / 16), db = first_b + s * (G::STAGE / 16);
+                tc_mma_f8(d, da, db, idesc, 0u);
+                tc_mma_f8(d, da + 2, db + 2, idesc, 1u);
+                tc_mma_f8(d, da + 4, db + 4, idesc, 1u);
+                tc_mma_f8(d, da + 6, db + 6, idesc, 1u);
+                tc_commit(&sum_full[buf]);
+                tc_commit(&empty[s]);
             }
+            __syncwarp();
+            if (++s == G::STAGES)
+            {
+                s = 0;
+                turn ^= 1;
+            }
+        }
+        if (!ok)
+        {
+            if (elect_one())
+                tc_commit(&drained);
+            __syncwarp();
+            mbar_wait(&drained, 0, status, 107);
         }
     }
     else
     {
-        // ---- scales: the product of a row's and the weights' scale, by block and row
-        constexpr int ROWS = (BN + 31) / 32;
         const int chunks = (n + G::CHUNK - 1) / G::CHUNK;
-        const float *sw = a.filt_scales + (size_t)kt * a.blocks + b0;
         for (int c = 0; c < chunks; ++c)
         {
-            float v[ROWS][G::CHUNK];
-#pragma unroll
-            for (int q = 0; q < ROWS; ++q)
-            {
-                const int col = q * 32 + lane, row = r0 + col;
-                const float *sx = a.in_scales + (size_t)row * a.blocks + b0;
-#pragma unroll
-                for (int j = 0; j < G::CHUNK; ++j)
-                {
-                    const int b = c * G::CHUNK + j;
-                    v[q][j] = col < BN && row < a.rows && b < n ? __ldg(sx + b) * __ldg(sw + b) : 0.f;
-                }
-            }
-            bool ok = c < 2 || mbar_wait(&sc_empty[c & 1], ((c >> 1) - 1) & 1, status, 108);
+            if (c > 0)
+                ask(c);
+            const bool ok = c < 2 || mbar_wait(&sc_empty[c & 1], ((c >> 1) - 1) & 1, status, 108);
             if (!__all_sync(0xffffffffu, ok))
                 break;
 #pragma unroll
@@ -237,7 +315,7 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
 #pragma unroll
                 for (int j = 0; j < G::CHUNK; ++j)
                     if (q * 32 + lane < BN)
-                        scales[((c & 1) * G::CHUNK + j) * BN + q * 32 + lane] = v[q][j];
+                        scales[((c & 1) * G::CHUNK + j) * BN + q * 32 + lane] = sv[q][j];
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(&sc_full[c & 1]);
@@ -245,60 +323,54 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
     }
     __syncwarp();
 
-    // ---- the cluster's parts, then bias, activation and the one rounding
-    const int k = kt * 128 + tid;
-    auto finish = [&](int col, float v) {
-        const int row = r0 + col;
-        if (row >= a.rows || k >= a.K)
-            return;
-        const long long at = (long long)row * a.out_stride + k;
-        if (a.accumulate)
-            v += load1<TYPE>(a.out, at);
-        if (a.bias)
-            v += __ldg(a.bias + k);
-        store1<TYPE>(a.out, at, activate(v, a.neg_scale));
-    };
-    if (a.split == 1)
+    // ---- every CTA of the cluster has a share of the rows: the others send it what they have of them (a wait that gave up leaves rubbish, which
+    // the status word tells)
+    cluster_wait(); // all inboxes can be written to
+    const int per = BN / a.split;
+    if (warp < 4)
     {
-        if (warp < 4)
-        {
+        int to = 0, pair = 0; // c = to * per + 2 * pair
 #pragma unroll
-            for (int c = 0; c < BN; ++c)
-                finish(c, acc[c]);
-        }
-    }
-    else
-    {
-        float *red = reinterpret_cast<float *>(ring); // [BN][128]
-        if (warp < 4)
+        for (int c = 0; c < BN; c += 2)
         {
-#pragma unroll
-            for (int c = 0; c < BN; ++c)
-                red[c * 128 + tid] = acc[c];
-        }
-        cluster_sync_all();
-        if (warp < 4)
-        {
-            const int per = BN / a.split;
-            for (int c = rank * per; c < rank * per + per && r0 + c < a.rows; ++c)
+            st_async_b64(map_to_cta(inbox + (rank * (per / 2) + pair) * 128 + tid, to), acc[c / 2], map_to_cta(&delivered, to));
+            if (2 * ++pair == per)
             {
-                float v = 0.f;
-                for (int q = 0; q < a.split; ++q)
-                {
-                    float p;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p) : "r"(map_to_cta(red + c * 128 + tid, q)));
-                    v += p;
-                }
-                finish(c, v);
+                pair = 0;
+                ++to;
             }
         }
-        __syncwarp();
-        cluster_sync_all(); // nobody's shared memory goes while it is read
     }
+    __syncwarp();
+    cluster_arrive_relaxed(); // nothing more is sent
+    const bool all = mbar_wait_cluster(&delivered, 0, status, 109);
+    // the parts in the order of the reduction, then bias, activation and the one rounding: a warp takes two rows, a lane four outputs
+    const int k = kt * 128 + 4 * lane;
+    for (int p = warp; 2 * p < per; p += FEW_THREADS / 32)
+    {
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+        for (int q = 0; q < a.split; ++q)
+        {
+            const float4 *in = reinterpret_cast<const float4 *>(inbox + (q * (per / 2) + p) * 128 + 4 * lane);
+            const float4 x = in[0], y = in[1];
+            u.x += x.x; v.x += x.y; u.y += x.z; v.y += x.w;
+            u.z += y.x; v.z += y.y; u.w += y.z; v.w += y.w;
+        }
+        const int row = r0 + rank * per + 2 * p;
+        if (k < a.K && row < a.rows)
+            finish4<TYPE>(a, row, k, u);
+        if (k < a.K && row + 1 < a.rows)
+            finish4<TYPE>(a, row + 1, k, v);
+    }
+    __syncwarp();
+    cluster_wait(); // this CTA's shared memory stays while anybody may send to it
+    if (!all)
+        for (int i = 0; i < 1000; ++i)
+            __nanosleep(1000); // and what was sent last is on its way for less than that
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 5)
-        tmem_dealloc(tmem, G::COLS < 32 ? 32 : G::COLS);
+        tmem_dealloc(tmem, G::COLS);
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -324,20 +396,12 @@ __device__ __forceinline__ TileAt tile_at(const DenseArgs &a, int t)
     return {(g * GROUP + in - kt * size) * 256, kt * MANY_N};
 }
 
-// Two sums times one scale onto two more, one instruction.
-__device__ __forceinline__ void fold2(unsigned long long &acc, uint32_t lo, uint32_t hi, unsigned long long s2)
-{
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(r), "l"(s2));
-}
 __device__ __forceinline__ void fold32(unsigned long long *acc, const uint32_t *r, unsigned long long s2)
 {
 #pragma unroll
     for (int c = 0; c < 16; ++c)
         fold2(acc[c], r[2 * c], r[2 * c + 1], s2);
 }
-__device__ __forceinline__ float2 pair_of(unsigned long long v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
 
 template <int TYPE>
 __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -646,9 +710,15 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
     if (!status)
         return fail(SMALL_B200_CUDA_ERROR, "device status word not available");
     CUtensorMap map_w, map_x;
-    if (D->rows <= 128)
+    // Microseconds that either kernel takes, fitted to 91 sizes (1 to 2048 rows, 512 to 8192 outputs and inputs): a tile and block of 128 outputs by 64 rows
+    // costs the device 2.6 ns in the one, a block of a wave of 256 x 256 tiles 0.48 us in the other.
+    // 256 rows, 4096 -> 4096: 16.4 and 20.0 us; 512 rows: 25.4 and 20.7; 256 rows, 8192 -> 1024: 12.1 and 32.9; 1024 rows: 24.9 and 33.3.
+    const double units = (double)((D->K + 127LL) / 128) * ((D->rows + 63LL) / 64) * a.blocks;
+    const long long pairs_of_tiles = ((D->K + 255LL) / 256) * ((D->rows + 255LL) / 256), at_once = std::max(1, num_sms() / 2);
+    const double many_us = (double)((pairs_of_tiles + at_once - 1) / at_once) * (0.48 * a.blocks + 1.2);
+    if (D->rows <= 64 || 0.0026 * units < many_us)
     {
-        const int bn = D->rows <= 16 ? 16 : D->rows <= 32 ? 32 : D->rows <= 64 ? 64 : 128;
+        const int bn = D->rows <= 16 ? 16 : D->rows <= 32 ? 32 : 64;
         a.k_tiles = (D->K + 127) / 128;
         a.r_tiles = (D->rows + bn - 1) / bn;
         // Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each at least two blocks.
@@ -663,8 +733,7 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
         {
         case 16: return launch_few<16, TYPE>(a, map_w, map_x, status, st);
         case 32: return launch_few<32, TYPE>(a, map_w, map_x, status, st);
-        case 64: return launch_few<64, TYPE>(a, map_w, map_x, status, st);
-        default: return launch_few<128, TYPE>(a, map_w, map_x, status, st);
+        default: return launch_few<64, TYPE>(a, map_w, map_x, status, st);
         }
     }
     a.k_tiles = (D->K + MANY_N - 1) / MANY_N;

@@ -138,6 +138,25 @@ __device__ __forceinline__ void cluster_sync_all()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The barrier's two halves, for work in between.  Every thread of the cluster arrives and waits; a relaxed arrival says no more than that this thread has come
+// this far (a release waits until its stores to global memory are performed, a microsecond).
+__device__ __forceinline__ void cluster_arrive_release()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_arrive_relaxed()
+{
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait()
+{
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Eight bytes into a CTA's shared memory, counted by a barrier of that CTA.
+__device__ __forceinline__ void st_async_b64(uint32_t cluster_addr, unsigned long long v, uint32_t cluster_bar)
+{
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(cluster_addr), "l"(v), "r"(cluster_bar) : "memory");
+}
 // Address of the same shared-memory location in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_to_cta(const void *p, uint32_t rank)
 {
