@@ -3,8 +3,7 @@
 //
 // Mathematics: scale = max|x| / 448 (448 is e4m3's largest value), code = x / scale to the nearest e4m3 value, ties to even, of the exact
 // quotient.  A product with the rounded inverse is up to 2^-22 off, which matters only next to the middle between two codes (bf16 data meets
-// middles exactly): both ends of that interval are converted, and only where the codes differ is x compared with middle * scale, exactly, in 64
-// bits.
+// middles): both ends of that interval are converted, and only where the codes differ is x compared with middle * scale, exactly.
 //
 // Bound: memory (2 or 4 bytes read and one written an element).  16 lanes own 8 columns each of a block, so the largest magnitude of a row block is
 // four shuffles away and nothing is read twice.
@@ -35,41 +34,63 @@ __device__ __forceinline__ float from_e4m3(uint32_t code)
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
     return __half2float(__ushort_as_half((unsigned short)(h & 0xffffu)));
 }
-// The code of x / scale where `near` and `far` (same sign, |near| <= |far|) are the two candidates.
+// The code of x / scale where `near` and `far` (same sign, |near| < |far|) are the two candidates: |x| against middle * scale, which is the float
+// `at` and what its rounding left.  Powers of two keep that remainder a normal number.
 __device__ __noinline__ uint32_t exact_code(float x, float scale, uint32_t near, uint32_t far)
 {
-    if (near == far)
-        return near;
-    const double middle = 0.5 * ((double)fabsf(from_e4m3(near)) + (double)fabsf(from_e4m3(far))); // five significant bits
-    const double ax = fabs((double)x), at = middle * (double)scale;                               // exact: 5 + 24 bits
+    const float up = scale < 1.f ? 1.8446744e19f : 1.f; // 2^64
+    const float middle = 0.5f * (fabsf(from_e4m3(near)) + fabsf(from_e4m3(far))), s = scale * up, ax = fabsf(x) * up;
+    const float at = middle * s, rest = fmaf(middle, s, -at); // middle has five significant bits
     if (ax != at)
         return ax < at ? near : far;
+    if (rest != 0.f)
+        return rest > 0.f ? near : far;
     return (near & 1u) ? far : near;
 }
-// Eight values to eight codes; inv is 1 / scale to within one rounding.
+// Two products with one factor, one instruction.
+__device__ __forceinline__ void mul2(float x, float y, unsigned long long f2, float &a, float &b)
+{
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(f2));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long twice(float f) { return (unsigned long long)__float_as_uint(f) << 32 | __float_as_uint(f); }
+// Eight values to eight codes; inv is 1 / scale to within 2^-23 of it.
 __device__ __forceinline__ uint2 quantize8(const float *x, float scale, float inv)
 {
-    constexpr float EPS = 4.76837158e-7f; // 2^-21: more than the product's and the inverse's roundings together
+    constexpr float EPS = 4.76837158e-7f; // 2^-21: more than the product's and the inverse's errors together
+    const unsigned long long below = twice(inv * (1.f - EPS)), above = twice(inv * (1.f + EPS));
     uint32_t n[4], f[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
-        const float a = x[2 * i] * inv, b = x[2 * i + 1] * inv;
-        n[i] = to_e4m3x2(a * (1.f - EPS), b * (1.f - EPS));
-        f[i] = to_e4m3x2(a * (1.f + EPS), b * (1.f + EPS));
+        float a, b;
+        mul2(x[2 * i], x[2 * i + 1], below, a, b);
+        n[i] = to_e4m3x2(a, b);
+        mul2(x[2 * i], x[2 * i + 1], above, a, b);
+        f[i] = to_e4m3x2(a, b);
     }
     uint32_t lo = n[0] | n[1] << 16, hi = n[2] | n[3] << 16;
     const uint32_t flo = f[0] | f[1] << 16, fhi = f[2] | f[3] << 16;
-    if (lo != flo || hi != fhi)
+    uint32_t dlo = lo ^ flo, dhi = hi ^ fhi;
+    while (dlo | dhi) // one in 250 bf16 values: fractions of small numbers lie next to middles
     {
-        uint32_t l = 0, h = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
+        const bool second = dlo == 0u;
+        const int at = (__ffs((int)(second ? dhi : dlo)) - 1) & 24;
+        const float p = second ? (at & 16 ? (at & 8 ? x[7] : x[6]) : (at & 8 ? x[5] : x[4]))
+                               : (at & 16 ? (at & 8 ? x[3] : x[2]) : (at & 8 ? x[1] : x[0]));
+        const uint32_t code = exact_code(p, scale, (second ? hi : lo) >> at & 0xffu, (second ? fhi : flo) >> at & 0xffu) << at, byte = 0xffu << at;
+        if (second)
         {
-            l |= exact_code(x[i], scale, lo >> (8 * i) & 0xffu, flo >> (8 * i) & 0xffu) << (8 * i);
-            h |= exact_code(x[4 + i], scale, hi >> (8 * i) & 0xffu, fhi >> (8 * i) & 0xffu) << (8 * i);
+            hi = (hi & ~byte) | code;
+            dhi &= ~byte;
         }
-        lo = l; hi = h;
+        else
+        {
+            lo = (lo & ~byte) | code;
+            dlo &= ~byte;
+        }
     }
     return make_uint2(lo, hi);
 }
@@ -88,7 +109,21 @@ __device__ __forceinline__ void infinities_to_nan(float *x)
     for (int i = 0; i < 8; ++i)
         x[i] = fabsf(x[i]) == INFINITY ? NAN : x[i];
 }
-__device__ __forceinline__ float scale_of(float amax) { return amax > 0.f ? fmaxf(__fdiv_rn(amax, F8_MAX), SCALE_MIN) : 1.f; }
+// amax / 448, rounded to nearest: the product with the rounded inverse and one correction by its exact remainder give every quotient from 2^-126 on
+// (all 2^23 significands of a dozen exponents were compared), in a sixth of a division's instructions.
+__device__ __forceinline__ float scale_of(float amax)
+{
+    constexpr float INV = 1.f / F8_MAX;
+    const float s = amax * INV, rest = fmaf(-s, F8_MAX, amax);
+    return amax > 0.f ? fmaxf(fmaf(rest, INV, s), SCALE_MIN) : 1.f;
+}
+// 1 / scale to within 2^-23 of it; scale is at least 2^-126 and below 2^120.
+__device__ __forceinline__ float inverse_of(float scale)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+    return r;
+}
 
 struct QuantArgs
 {
@@ -98,54 +133,140 @@ struct QuantArgs
     FastDiv by_blocks;
 };
 
-constexpr int ROW_THREADS = 256, UNITS = 2; // row blocks that 16 lanes have in flight
-
-template <int TYPE, bool VEC>
-__global__ void __launch_bounds__(ROW_THREADS) quantize_rows_f8_kernel(const QuantArgs a, const void *__restrict__ in, uint8_t *__restrict__ out,
-                                                                         float *__restrict__ scales)
+// Eight elements as they are in memory; zeros where there are none.
+template <int TYPE>
+struct Raw8
 {
-    constexpr int GROUPS = ROW_THREADS / 16;
-    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
-    // all lanes of a warp stay in the loop together: the shuffles need them
-    for (long long u0 = (long long)blockIdx.x * (GROUPS * UNITS); u0 < a.units; u0 += (long long)gridDim.x * (GROUPS * UNITS))
+    uint4 w[TYPE == SMALL_B200_TYPE_F32 ? 2 : 1];
+    template <bool VEC>
+    __device__ __forceinline__ void load(const void *p, long long at, bool has)
     {
-        float x[UNITS][8];
-        int row[UNITS], block[UNITS];
-        bool has[UNITS];
-#pragma unroll
-        for (int j = 0; j < UNITS; ++j)
+        constexpr int N = TYPE == SMALL_B200_TYPE_F32 ? 2 : 1, SIZE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 2;
+        if (VEC)
         {
-            const long long u = u0 + j * GROUPS + group;
-            row[j] = u < a.units ? a.by_blocks.div((int)u) : 0;
-            block[j] = u < a.units ? (int)u - row[j] * a.blocks : 0;
-            const int c = block[j] * 128 + lane * 8;
-            has[j] = u < a.units && c < a.columns;
-            load8<TYPE, VEC>(in, (long long)row[j] * a.stride + c, has[j], x[j]);
+            const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const char *>(p) + at * SIZE);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                w[i] = has ? __ldg(q + i) : make_uint4(0u, 0u, 0u, 0u);
+            return;
         }
+        uint32_t v[4 * N];
 #pragma unroll
-        for (int j = 0; j < UNITS; ++j)
+        for (int i = 0; i < 4 * N; ++i)
+            if (SIZE == 4)
+                v[i] = has ? __ldg(static_cast<const uint32_t *>(p) + at + i) : 0u;
+            else
+                v[i] = has ? __ldg(static_cast<const uint16_t *>(p) + at + 2 * i) | (uint32_t)__ldg(static_cast<const uint16_t *>(p) + at + 2 * i + 1) << 16 : 0u;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            w[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+    __device__ __forceinline__ void unpack(float *x) const
+    {
+        if (TYPE == SMALL_B200_TYPE_F32)
         {
-            float m = abs_max8(x[j]);
-#pragma unroll
-            for (int d = 8; d > 0; d >>= 1)
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            if (__any_sync(0xffffffffu, m == INFINITY)) // rare
-            {
-                infinities_to_nan(x[j]);
-                m = abs_max8(x[j]);
-#pragma unroll
-                for (int d = 8; d > 0; d >>= 1)
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-            }
-            const float scale = scale_of(m);
-            if (has[j])
-            {
-                *reinterpret_cast<uint2 *>(out + (long long)row[j] * a.columns + block[j] * 128 + lane * 8) = quantize8(x[j], scale, __frcp_rn(scale));
-                if (lane == 0)
-                    scales[(long long)row[j] * a.blocks + block[j]] = scale;
-            }
+            const uint4 &a = w[0], &b = w[TYPE == SMALL_B200_TYPE_F32 ? 1 : 0];
+            x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+            x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
+        }
+        else
+        {
+            unpack2<TYPE>(w[0].x, x[0], x[1]); unpack2<TYPE>(w[0].y, x[2], x[3]); unpack2<TYPE>(w[0].z, x[4], x[5]); unpack2<TYPE>(w[0].w, x[6], x[7]);
         }
     }
+};
+// The largest magnitude of the 16 lanes' values; a NaN is not seen.
+template <int TYPE>
+__device__ __forceinline__ float block_max(const Raw8<TYPE> &r, const float *x)
+{
+    if (TYPE == SMALL_B200_TYPE_F32)
+    {
+        float m = abs_max8(x);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1)
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        return m;
+    }
+    // two at a time, as they are
+    auto max2 = [](uint32_t a, uint32_t b) {
+        uint32_t c;
+        if (TYPE == SMALL_B200_TYPE_BF16)
+            asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+        else
+            asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+        return c;
+    };
+    constexpr uint32_t MAG = 0x7fff7fffu;
+    uint32_t m = max2(max2(r.w[0].x & MAG, r.w[0].y & MAG), max2(r.w[0].z & MAG, r.w[0].w & MAG));
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1)
+        m = max2(m, __shfl_xor_sync(0xffffffffu, m, d));
+    float lo, hi;
+    unpack2<TYPE>(m, lo, hi);
+    return fmaxf(fmaxf(lo, hi), 0.f); // 0 where all are NaN
+}
+// A row block's codes and scale.
+template <int TYPE>
+__device__ __forceinline__ void finish_block(const Raw8<TYPE> &r, bool has, uint8_t *codes, float *scale_at, int lane)
+{
+    float x[8];
+    r.unpack(x);
+    float m = block_max<TYPE>(r, x);
+    if (__any_sync(0xffffffffu, m == INFINITY)) // rare
+    {
+        infinities_to_nan(x);
+        m = abs_max8(x);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1)
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    }
+    const float scale = scale_of(m);
+    if (has)
+    {
+        *reinterpret_cast<uint2 *>(codes) = quantize8(x, scale, inverse_of(scale));
+        if (lane == 0)
+            *scale_at = scale;
+    }
+}
+
+constexpr int ROW_THREADS = 256, GROUPS = ROW_THREADS / 16, UNITS = 4; // row blocks at a time, and how many of them 16 lanes have in flight
+
+// FLAT: packed rows of whole blocks, so that block u is elements 128 u to 128 u + 127 and scale u.
+template <int TYPE, bool VEC, bool FLAT>
+__global__ void __launch_bounds__(ROW_THREADS, TYPE == SMALL_B200_TYPE_F32 ? 4 : 5)
+    quantize_rows_f8_kernel(const QuantArgs a, const void *__restrict__ in, uint8_t *__restrict__ out, float *__restrict__ scales)
+{
+    constexpr int SIZE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 2;
+    const int lane = threadIdx.x & 15;
+    const long long u0 = (long long)blockIdx.x * (GROUPS * UNITS) + (threadIdx.x >> 4);
+    Raw8<TYPE> r[UNITS];
+    if (FLAT && ((long long)blockIdx.x + 1) * (GROUPS * UNITS) <= a.units)
+    {
+        const char *p = static_cast<const char *>(in) + (u0 * 128 + lane * 8) * SIZE;
+        uint8_t *q = out + u0 * 128 + lane * 8;
+#pragma unroll
+        for (int j = 0; j < UNITS; ++j)
+            r[j].template load<VEC>(p + j * GROUPS * 128 * SIZE, 0, true);
+#pragma unroll
+        for (int j = 0; j < UNITS; ++j)
+            finish_block<TYPE>(r[j], true, q + j * GROUPS * 128, scales + u0 + j * GROUPS, lane);
+        return;
+    }
+    long long to[UNITS]; // where a lane's eight codes are
+    bool has[UNITS];
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j)
+    {
+        const long long u = u0 + j * GROUPS;
+        has[j] = u < a.units;
+        const int row = has[j] ? a.by_blocks.div((int)u) : 0, c = has[j] ? ((int)u - row * a.blocks) * 128 + lane * 8 : 0;
+        has[j] = has[j] && c < a.columns;
+        to[j] = (long long)row * a.columns + c;
+        r[j].template load<VEC>(in, (long long)row * a.stride + c, has[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) // all lanes of a warp together: the shuffles need them
+        finish_block<TYPE>(r[j], has[j], out + to[j], scales + u0 + j * GROUPS, lane);
 }
 
 // A CTA owns a square block: 16 lanes by 16 rows at a time, eight times, all of it in registers.
@@ -189,7 +310,7 @@ __global__ void __launch_bounds__(256) quantize_square_f8_kernel(const QuantArgs
             __syncthreads();
             continue;
         }
-        const float scale = scale_of(m), inv = __frcp_rn(scale);
+        const float scale = scale_of(m), inv = inverse_of(scale);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
         {
@@ -211,9 +332,11 @@ int launch_quantize(const QuantArgs &a, int block_rows, const void *in, uint8_t 
         quantize_square_f8_kernel<TYPE, VEC><<<(unsigned)a.units, 256, 0, st>>>(a, in, out, scales);
         return launched("quantize_square_f8_kernel");
     }
-    long long blocks = (a.units + ROW_THREADS / 16 * UNITS - 1) / (ROW_THREADS / 16 * UNITS);
-    const long long most = (long long)num_sms() * 16;
-    quantize_rows_f8_kernel<TYPE, VEC><<<(unsigned)(blocks < most ? blocks : most), ROW_THREADS, 0, st>>>(a, in, out, scales);
+    const unsigned grid = (unsigned)((a.units + GROUPS * UNITS - 1) / (GROUPS * UNITS));
+    if (VEC && a.stride == a.columns && a.columns % 128 == 0)
+        quantize_rows_f8_kernel<TYPE, VEC, VEC><<<grid, ROW_THREADS, 0, st>>>(a, in, out, scales);
+    else
+        quantize_rows_f8_kernel<TYPE, VEC, false><<<grid, ROW_THREADS, 0, st>>>(a, in, out, scales);
     return launched("quantize_rows_f8_kernel");
 }
 } // namespace

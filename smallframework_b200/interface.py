@@ -651,29 +651,44 @@ def Conv2D_ReLU_DepthwiseConv2D_ReLU(conv_kernel_height, conv_kernel_width, conv
 
 
 # --------------------------------------------------------------------------- narrow types
-def _narrow(name, buf, elems, what, types=None):
-    """Address of a buffer's (or a flat tensor's) elements: of an allowed type, on the current device, `elems` of them at least."""
-    t = buf.t if isinstance(buf, (FloatBuffer, _NarrowBuffer)) else buf
-    if not t.is_cuda:
+def _home(name, t, what):
+    """The current device's number, which is the tensor's too."""
+    here = t.get_device()
+    if here < 0:
         raise _lib.SmallB200Error("buffers must live on a CUDA device (no CPU path)")
-    if t.dtype not in (types or _TYPES):
-        raise ValueError(f"{name}: {what} of type {t.dtype}")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name}: {what} on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    if not t.is_contiguous():
+    now = _device() if _device is not None else torch.cuda.current_device()
+    if here != now:
+        raise ValueError(f"{name}: {what} on cuda:{here}, the current device is cuda:{now}")
+    return here
+
+
+def _at(name, t, elems, what, types, here):
+    """Address of a flat tensor's elements: of an allowed type, on the current device, `elems` of them at least."""
+    if t.get_device() != here or t.dtype not in types or t.numel() < elems or not t.is_contiguous():
+        if not t.is_cuda:
+            raise _lib.SmallB200Error("buffers must live on a CUDA device (no CPU path)")
+        if t.get_device() != here:
+            raise ValueError(f"{name}: {what} on {t.device}, the others are on cuda:{here}")
+        if t.dtype not in types:
+            raise ValueError(f"{name}: {what} of type {t.dtype}")
+        if t.numel() < elems:
+            raise ValueError(f"{name}: {what} holds {t.numel()} elements, {elems} needed")
         raise ValueError(f"{name}: {what} is not contiguous")
-    if t.numel() < elems:
-        raise ValueError(f"{name}: {what} holds {t.numel()} elements, {elems} needed")
     return t.data_ptr()
 
 
-def _sizes(name, *numbers):
-    for n in numbers:
-        if not 0 <= n < 1 << 31:  # a longer one would lose its upper bits on the way to the library
-            raise ValueError(f"{name}: a size of {n}")
+def _tensor(buf):
+    """Layers of narrow types take a buffer or, like a bias of the other layers, a flat tensor."""
+    return buf if isinstance(buf, torch.Tensor) else buf.t
+
+
+def _size(name, n):
+    if not 0 <= n < 1 << 31:  # a longer one would lose its upper bits on the way to the library
+        raise ValueError(f"{name}: a size of {n}")
 
 
 _F32, _F8, _TOKENS, _I32 = (torch.float32,), (torch.float8_e4m3fn,), (torch.int32, torch.int64), (torch.int32,)
+_FLOATS = tuple(_TYPES)
 
 
 def QuantizeBlocks(num_rows, num_columns, input_buf, output_buf, *, input_stride=None, stream=None):
@@ -685,13 +700,15 @@ def QuantizeBlocks(num_rows, num_columns, input_buf, output_buf, *, input_stride
         raise ValueError(f"{name}: the output is a Float8Buffer")
     if (output_buf.rows, output_buf.columns) != (num_rows, num_columns):
         raise ValueError(f"{name}: an output of {output_buf.rows} x {output_buf.columns} for {num_rows} x {num_columns}")
-    _sizes(name, num_rows, num_columns)
+    _size(name, num_rows)
+    _size(name, num_columns)
     apart = num_columns if input_stride is None else input_stride
-    x = _narrow(name, input_buf, (num_rows - 1) * apart + num_columns if num_rows > 0 else 0, "input")
-    kind = _TYPES[input_buf.t.dtype]
-    check(lib().small_b200_quantize_blocks_f8(num_rows, num_columns, output_buf.block_rows, kind, x, apart,
-                                              _narrow(name, output_buf, 0, "output", _F8), _narrow(name, output_buf.scales, 0, "scales", _F32),
-                                              _stream(stream)))
+    x = _tensor(input_buf)
+    here = _home(name, x, "input")
+    at = _at(name, x, (num_rows - 1) * apart + num_columns if num_rows > 0 else 0, "input", _FLOATS, here)
+    check(lib().small_b200_quantize_blocks_f8(num_rows, num_columns, output_buf.block_rows, _TYPES[x.dtype], at, apart,
+                                              _at(name, output_buf.t, num_rows * num_columns, "output", _F8, here),
+                                              _at(name, output_buf.scales, -(-num_rows // output_buf.block_rows) * -(-num_columns // 128), "scales", _F32, here), _stream(stream)))
 
 
 def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, out_stride, stream):
@@ -701,15 +718,19 @@ def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, o
         raise ValueError(f"{name}: activations in blocks of 1 row and weights in blocks of 128, not {inp.block_rows} and {filt.block_rows}")
     if (filt.rows, filt.columns) != (K, C_) or inp.columns != C_ or inp.rows < rows:
         raise ValueError(f"{name}: weights {filt.rows} x {filt.columns} and activations {inp.rows} x {inp.columns} for {rows} rows, {C_} -> {K}")
-    if not isinstance(out, (FloatBuffer, BFloat16Buffer, HalfBuffer)) or out.t.dtype not in _TYPES:
+    y = _tensor(out)
+    if y.dtype not in _FLOATS:
         raise ValueError(f"{name}: the output is a FloatBuffer, BFloat16Buffer or HalfBuffer")
-    _sizes(name, rows, K, C_)
+    _size(name, rows)
+    _size(name, K)
+    _size(name, C_)
     apart = K if out_stride is None else out_stride
-    L = _dense_layer(rows, K, C_, _TYPES[out.t.dtype], apart, accumulate, act, slope)
-    check(lib().small_b200_dense_f8(L, _narrow(name, inp, 0, "input", _F8), _narrow(name, inp.scales, 0, "input scales", _F32),
-                                    _narrow(name, filt, 0, "filter", _F8), _narrow(name, filt.scales, 0, "filter scales", _F32),
-                                    None if bias is None else _narrow(name, bias, K, "bias", _F32),
-                                    _narrow(name, out, (rows - 1) * apart + K if rows > 0 else 0, "output"), _stream(stream)))
+    L = _dense_layer(rows, K, C_, _TYPES[y.dtype], apart, accumulate, act, slope)
+    blocks, here = -(-C_ // 128), _home(name, y, "output")
+    check(lib().small_b200_dense_f8(L, _at(name, inp.t, rows * C_, "input", _F8, here), _at(name, inp.scales, rows * blocks, "input scales", _F32, here),
+                                    _at(name, filt.t, K * C_, "filter", _F8, here), _at(name, filt.scales, -(-K // 128) * blocks, "filter scales", _F32, here),
+                                    None if bias is None else _at(name, _tensor(bias), K, "bias", _F32, here),
+                                    _at(name, y, (rows - 1) * apart + K if rows > 0 else 0, "output", _FLOATS, here), _stream(stream)))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -729,16 +750,21 @@ def LogProbabilities(num_rows, num_classes, logits_buf, tokens, logprobs_buf, en
     with logprobs_buf).  Classes at minus infinity are masked; a row with nothing else has log-probabilities of minus infinity and an entropy of 0.
     A row with NaN or plus infinity has NaN for both.  small::SoftMax (:1778 of the reference) subtracts no maximum and knows no classes."""
     name = "LogProbabilities"
-    _sizes(name, num_rows, num_classes, top)
+    _size(name, num_rows)
+    _size(name, num_classes)
+    _size(name, top)
     apart = num_classes if row_stride is None else row_stride
-    x = _narrow(name, logits_buf, (num_rows - 1) * apart + num_classes if num_rows > 0 else 0, "logits")
-    given = None if tokens is None else _narrow(name, tokens, num_rows, "tokens", _TOKENS)
+    x = _tensor(logits_buf)
+    here = _home(name, x, "logits")
+    at = _at(name, x, (num_rows - 1) * apart + num_classes if num_rows > 0 else 0, "logits", _FLOATS, here)
+    each = num_rows * top
     check(lib().small_b200_logprobs(
-        num_rows, num_classes, _TYPES[logits_buf.t.dtype], x, apart, 4 if tokens is None else tokens.element_size(), given,
-        None if logprobs_buf is None else _narrow(name, logprobs_buf, num_rows, "log-probabilities", _F32),
-        None if entropy_buf is None else _narrow(name, entropy_buf, num_rows, "entropy", _F32), top,
-        None if top_logprobs_buf is None else _narrow(name, top_logprobs_buf, num_rows * top, "top log-probabilities", _F32),
-        None if top_tokens is None else _narrow(name, top_tokens, num_rows * top, "top tokens", _I32), _stream(stream)))
+        num_rows, num_classes, _TYPES[x.dtype], at, apart, 4 if tokens is None else tokens.element_size(),
+        None if tokens is None else _at(name, tokens, num_rows, "tokens", _TOKENS, here),
+        None if logprobs_buf is None else _at(name, _tensor(logprobs_buf), num_rows, "log-probabilities", _F32, here),
+        None if entropy_buf is None else _at(name, _tensor(entropy_buf), num_rows, "entropy", _F32, here), top,
+        None if top_logprobs_buf is None else _at(name, _tensor(top_logprobs_buf), each, "top log-probabilities", _F32, here),
+        None if top_tokens is None else _at(name, top_tokens, each, "top tokens", _I32, here), _stream(stream)))
 
 
 # --------------------------------------------------------------------------- detection head
