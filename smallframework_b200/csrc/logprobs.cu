@@ -2,7 +2,7 @@
 //
 // Mathematics, for a row x: m = max x, t_i = x_i - m, S = sum e^t_i, T = sum t_i e^t_i;
 //   log p_i = t_i - log S,   H = -sum p_i log p_i = log S - T / S  (both terms non-negative: no cancellation).
-// Every thread keeps (m, S, T) of the vectors it has read and rescales when its maximum moves; pairs merge as S = sum S_j e^(m_j - m),
+// Every thread keeps (m, S, T) of the vectors it has read and rescales when its maximum has moved far; pairs merge as S = sum S_j e^(m_j - m),
 // T = sum (T_j + S_j (m_j - m)) e^(m_j - m).  A masked class (minus infinity, or a value so low that its exponential is 0) adds 0 to both.
 //
 // Best alternatives: a thread also remembers which of its vectors first held its maximum.  These (value, vector) keys are all different, and the
@@ -22,7 +22,7 @@ using namespace sb;
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, TOP_MOST = 32, MAX_SPLIT = 8;
 constexpr int CANDIDATES = 1024;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, SLACK = 4.f;
 
 struct LogpArgs
 {
@@ -54,6 +54,33 @@ __device__ __forceinline__ float value_of(uint32_t order)
     return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
 }
 __device__ __forceinline__ unsigned long long make_key(uint32_t order, uint32_t index) { return (unsigned long long)order << 32 | (0xffffffffu - index); }
+
+// Pairs of floats, one instruction for both.
+__device__ __forceinline__ unsigned long long pair(float x, float y)
+{
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void halves(unsigned long long v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b)
+{
+    unsigned long long v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b)
+{
+    unsigned long long v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c)
+{
+    unsigned long long v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
 
 struct Stats
 {
@@ -116,6 +143,25 @@ __device__ __forceinline__ void unpack_vector(const uint4 &w, float *x)
     }
 }
 
+// The largest of a vector's elements; a NaN is not seen (NaN where there is nothing else).
+template <int TYPE>
+__device__ __forceinline__ float vector_max(const uint4 &w, const float *x)
+{
+    if (TYPE == SMALL_B200_TYPE_F32)
+        return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    auto max2 = [](uint32_t a, uint32_t b) {
+        uint32_t c;
+        if (TYPE == SMALL_B200_TYPE_BF16)
+            asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+        else
+            asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+        return c;
+    };
+    float lo, hi;
+    unpack2<TYPE>(max2(max2(w.x, w.y), max2(w.z, w.w)), lo, hi);
+    return fmaxf(lo, hi);
+}
+
 // Descending order over the 32 lanes; FROM: the length of the bitonic runs the lanes hold already (2: none).
 template <int FROM>
 __device__ __forceinline__ unsigned long long sort_lanes(unsigned long long key, int lane)
@@ -176,46 +222,73 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, con
     const int share = (vectors + a.split - 1) / a.split;
     const int v0 = rank * share, v1 = min(vectors, v0 + share);
 
-    // ---- one pass: maximum and sums of this thread's vectors
-    float m = -INFINITY, mu = 0.f, S = 0.f, T = 0.f; // mu: m, or 0 while there is none
-    int at = v0 + tid;                               // the vector that held m first
-    for (int v = v0 + tid; v < v1; v += BATCH * THREADS)
+    // ---- one pass: maximum and sums of this thread's vectors.  The exponentials are relative to mu, which follows the maximum only when that is SLACK above
+    // it: at every step some lane of a warp has a new maximum, but one that matters is rare.
+    float m = -INFINITY, mu = 0.f, limit = -INFINITY; // limit: mu + SLACK, or minus infinity while there is no mu
+    unsigned long long S2 = 0ull, T2 = 0ull, minus_mu = 0ull;
+    const unsigned long long log2e2 = pair(LOG2E, LOG2E);
+    int at = v0 + tid; // the vector that held m first
+    auto add = [&](const uint4 &w, int v) {
+        float x[VE];
+        unpack_vector<TYPE>(w, x);
+        const float vm = vector_max<TYPE>(w, x);
+        if (vm > m)
+        {
+            m = vm;
+            at = v;
+        }
+        if (vm > limit)
+        {
+            if (limit != -INFINITY)
+            {
+                const float d = mu - vm, c = exp2_approx(d * LOG2E);
+                const unsigned long long c2 = pair(c, c);
+                T2 = c == 0.f ? 0ull : mul2(fma2(S2, pair(d, d), T2), c2);
+                S2 = mul2(S2, c2);
+            }
+            mu = vm;
+            limit = vm + SLACK;
+            minus_mu = pair(-mu, -mu);
+        }
+#pragma unroll
+        for (int i = 0; i < VE; i += 2)
+        {
+            float p, q;
+            halves(add2(pair(x[i], x[i + 1]), minus_mu), p, q);
+            const unsigned long long t = pair(max_nan(p, -1e30f), max_nan(q, -1e30f)); // finite: the exponential's 0 times it is 0
+            halves(mul2(t, log2e2), p, q);
+            const unsigned long long e = pair(exp2_approx(p), exp2_approx(q));
+            S2 = add2(S2, e);
+            T2 = fma2(e, t, T2);
+        }
+    };
+    int v = v0 + tid;
+    for (; v + (BATCH - 1) * THREADS < v1; v += BATCH * THREADS)
     {
         uint4 w[BATCH];
 #pragma unroll
         for (int j = 0; j < BATCH; ++j)
-            if (v + j * THREADS < v1)
-                w[j] = load_vector<TYPE>(row, v + j * THREADS, skew, a.classes);
+            w[j] = load_vector<TYPE>(row, v + j * THREADS, skew, a.classes);
 #pragma unroll
         for (int j = 0; j < BATCH; ++j)
-            if (v + j * THREADS < v1)
-            {
-                float x[VE];
-                unpack_vector<TYPE>(w[j], x);
-                float vm = x[0];
-#pragma unroll
-                for (int i = 1; i < VE; ++i)
-                    vm = fmaxf(vm, x[i]);
-                if (vm > m)
-                {
-                    if (m != -INFINITY)
-                    {
-                        const float d = m - vm, c = exp2_approx(d * LOG2E);
-                        T = c == 0.f ? 0.f : (T + S * d) * c;
-                        S *= c;
-                    }
-                    m = mu = vm;
-                    at = v + j * THREADS;
-                }
-#pragma unroll
-                for (int i = 0; i < VE; ++i)
-                {
-                    const float t = max_nan(x[i] - mu, -1e30f); // finite: the exponential's 0 times it is 0
-                    const float e = exp2_approx(t * LOG2E);
-                    S += e;
-                    T = fmaf(e, t, T);
-                }
-            }
+            add(w[j], v + j * THREADS);
+    }
+    for (; v < v1; v += THREADS)
+        add(load_vector<TYPE>(row, v, skew, a.classes), v);
+    // relative to the maximum itself
+    float S, T;
+    {
+        float p, q;
+        halves(S2, p, q);
+        S = p + q;
+        halves(T2, p, q);
+        T = p + q;
+        const float d = mu - m, c = exp2_approx(d * LOG2E);
+        if (m != -INFINITY)
+        {
+            T = (T + S * d) * c;
+            S *= c;
+        }
     }
     const bool any = v0 + tid < v1;
 
