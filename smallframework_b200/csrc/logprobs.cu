@@ -20,9 +20,9 @@ namespace
 {
 using namespace sb;
 
-constexpr int THREADS = 256, WARPS = THREADS / 32, TOP_MOST = 32, MAX_SPLIT = 8;
+constexpr int TOP_MOST = 32, MAX_SPLIT = 8;
 constexpr int CANDIDATES = 1024;
-constexpr float LOG2E = 1.4426950408889634f, SLACK = 4.f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, SLACK = 4.f;
 
 struct LogpArgs
 {
@@ -145,10 +145,10 @@ __device__ __forceinline__ void unpack_vector(const uint4 &w, float *x)
 
 // The largest of a vector's elements; a NaN is not seen (NaN where there is nothing else).
 template <int TYPE>
-__device__ __forceinline__ float vector_max(const uint4 &w, const float *x)
+__device__ __forceinline__ float vector_max(const uint4 &w)
 {
     if (TYPE == SMALL_B200_TYPE_F32)
-        return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
     auto max2 = [](uint32_t a, uint32_t b) {
         uint32_t c;
         if (TYPE == SMALL_B200_TYPE_BF16)
@@ -162,21 +162,38 @@ __device__ __forceinline__ float vector_max(const uint4 &w, const float *x)
     return fmaxf(lo, hi);
 }
 
-// Descending order over the 32 lanes; FROM: the length of the bitonic runs the lanes hold already (2: none).
-template <int FROM>
-__device__ __forceinline__ unsigned long long sort_lanes(unsigned long long key, int lane)
+// Masked classes in a row whose maximum is ordinary: within 1e6, so that its product with log2 e is rounded by less than 0.1, and in half precision
+// above -6e4, far enough from the type's lowest value.
+template <int TYPE>
+struct Masked
 {
-#pragma unroll
-    for (int run = FROM; run <= 32; run <<= 1)
-#pragma unroll
-        for (int d = run >> 1; d > 0; d >>= 1)
+    static constexpr float ORDINARY = TYPE == SMALL_B200_TYPE_F16 ? -6e4f : -1e6f;
+    // Minus infinity and what is as low become -1e38 (-65504 in half precision): finite, times log2 e too, and still with an exponential of 0.
+    __device__ __forceinline__ static void finite(uint4 &w, float *x)
+    {
+        if (TYPE == SMALL_B200_TYPE_F32)
         {
-            const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, d);
-            const bool keep_larger = ((lane & d) == 0) == ((lane & run) == 0 || run == 32);
-            key = keep_larger == (key > other) ? key : other;
+            unpack_vector<TYPE>(w, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[i] = max_nan(x[i], -1e38f);
+            return;
         }
-    return key;
-}
+        constexpr uint32_t LOWEST = TYPE == SMALL_B200_TYPE_BF16 ? 0xfe96fe96u : 0xfbfffbffu;
+        auto max2 = [](uint32_t a) {
+            uint32_t c;
+            if (TYPE == SMALL_B200_TYPE_BF16)
+                asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(LOWEST));
+            else
+                asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(LOWEST));
+            return c;
+        };
+        w = make_uint4(max2(w.x), max2(w.y), max2(w.z), max2(w.w));
+        unpack_vector<TYPE>(w, x);
+    }
+};
+
+template <int WARPS>
 __device__ __forceinline__ unsigned long long block_max(unsigned long long key, unsigned long long *part)
 {
 #pragma unroll
@@ -196,23 +213,26 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long key, 
     return key;
 }
 
+template <int WARPS>
 struct Shared
 {
     Stats part[WARPS], all;
-    unsigned long long sorted[WARPS][32];
-    unsigned long long best[TOP_MOST];                  // this CTA's best elements, in order
-    unsigned long long found[CANDIDATES];
-    unsigned long long merged[MAX_SPLIT * TOP_MOST];
+    unsigned long long bound[WARPS], last;
+    unsigned long long best[TOP_MOST]; // this CTA's best elements, in order
+    unsigned long long found[WARPS == 1 ? 256 : CANDIDATES];
+    unsigned long long merged[WARPS == 1 ? 1 : MAX_SPLIT * TOP_MOST];
+    int first[TOP_MOST]; // the best threads' first vectors
     int count;
 };
 
-template <int TYPE>
-__global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens,
+template <int TYPE, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens,
                                                             float *__restrict__ logprobs, float *__restrict__ entropy,
                                                             float *__restrict__ top_logprobs, int *__restrict__ top_tokens)
 {
-    constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, BATCH = 4;
-    __shared__ Shared sh;
+    constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, BATCH = 4, THREADS = 32 * WARPS;
+    constexpr int ROOM = sizeof(Shared<WARPS>::found) / 8;
+    __shared__ Shared<WARPS> sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long r = blockIdx.x / a.split;
     const int rank = (int)(blockIdx.x % a.split);
@@ -221,61 +241,119 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, con
     const int vectors = (int)(((long long)skew + a.classes + VE - 1) / VE);
     const int share = (vectors + a.split - 1) / a.split;
     const int v0 = rank * share, v1 = min(vectors, v0 + share);
+    // the given class's logit, asked for before everything else
+    long long token = -1;
+    float given = 0.f;
+    if (tid == 0 && rank == 0 && logprobs)
+    {
+        token = a.token_bytes == 8 ? static_cast<const long long *>(tokens)[r] : static_cast<const int *>(tokens)[r];
+        if (token >= 0 && token < a.classes)
+            given = load1<TYPE>(row, token);
+    }
 
-    // ---- one pass: maximum and sums of this thread's vectors.  The exponentials are relative to mu, which follows the maximum only when that is SLACK above
-    // it: at every step some lane of a warp has a new maximum, but one that matters is rare.
-    float m = -INFINITY, mu = 0.f, limit = -INFINITY; // limit: mu + SLACK, or minus infinity while there is no mu
-    unsigned long long S2 = 0ull, T2 = 0ull, minus_mu = 0ull;
+    // ---- one pass: maximum and sums of this thread's vectors, in powers of two: S = sum 2^(L x - R), T = sum (L x - R) 2^(L x - R), L = log2 e.  The
+    // reference R is L mu, rounded, and mu follows the maximum only when that is SLACK above it: at every step some lane of a warp has a new maximum, but
+    // one that matters is rare.  Where mu is beyond ORDINARY, L mu is not rounded but subtracted first (R = L mu, exactly).
+    float m = -INFINITY, mu = 0.f, R = 0.f, limit = -INFINITY; // limit: mu + SLACK, or minus infinity while there is no mu
+    bool ordinary = true;
+    unsigned long long S2 = 0ull, T2 = 0ull, minus_R = 0ull;
     const unsigned long long log2e2 = pair(LOG2E, LOG2E);
     int at = v0 + tid; // the vector that held m first
-    auto add = [&](const uint4 &w, int v) {
+    auto reference = [&](float vm) {
+        const bool now = vm > Masked<TYPE>::ORDINARY && vm < 1e6f;
+        const float to = vm * LOG2E;
+        if (limit != -INFINITY)
+        {
+            const float d = ordinary ? (now ? R - to : -fmaf(vm, LOG2E, -R)) : (now ? fmaf(mu, LOG2E, -to) : (mu - vm) * LOG2E), c = exp2_approx(d);
+            const unsigned long long c2 = pair(c, c);
+            T2 = c == 0.f ? 0ull : mul2(fma2(S2, pair(d, d), T2), c2);
+            S2 = mul2(S2, c2);
+        }
+        mu = vm; R = to; limit = vm + SLACK; ordinary = now;
+        minus_R = pair(-to, -to);
+    };
+    // One vector's terms; what masked classes become there has an exponential of 0 but is finite: 0 times minus infinity would be NaN.
+    auto add = [&](uint4 w) {
         float x[VE];
-        unpack_vector<TYPE>(w, x);
-        const float vm = vector_max<TYPE>(w, x);
-        if (vm > m)
-        {
-            m = vm;
-            at = v;
-        }
-        if (vm > limit)
-        {
-            if (limit != -INFINITY)
-            {
-                const float d = mu - vm, c = exp2_approx(d * LOG2E);
-                const unsigned long long c2 = pair(c, c);
-                T2 = c == 0.f ? 0ull : mul2(fma2(S2, pair(d, d), T2), c2);
-                S2 = mul2(S2, c2);
-            }
-            mu = vm;
-            limit = vm + SLACK;
-            minus_mu = pair(-mu, -mu);
-        }
+        Masked<TYPE>::finite(w, x);
 #pragma unroll
         for (int i = 0; i < VE; i += 2)
         {
+            const unsigned long long t = fma2(pair(x[i], x[i + 1]), log2e2, minus_R);
             float p, q;
-            halves(add2(pair(x[i], x[i + 1]), minus_mu), p, q);
-            const unsigned long long t = pair(max_nan(p, -1e30f), max_nan(q, -1e30f)); // finite: the exponential's 0 times it is 0
-            halves(mul2(t, log2e2), p, q);
+            halves(t, p, q);
             const unsigned long long e = pair(exp2_approx(p), exp2_approx(q));
             S2 = add2(S2, e);
             T2 = fma2(e, t, T2);
+        }
+    };
+    auto add_exactly = [&](const uint4 &w) {
+        float x[VE];
+        unpack_vector<TYPE>(w, x);
+#pragma unroll
+        for (int i = 0; i < VE; i += 2)
+        {
+            const float p = max_nan((x[i] - mu) * LOG2E, -1e30f), q = max_nan((x[i + 1] - mu) * LOG2E, -1e30f);
+            const unsigned long long e = pair(exp2_approx(p), exp2_approx(q));
+            S2 = add2(S2, e);
+            T2 = fma2(e, pair(p, q), T2);
         }
     };
     int v = v0 + tid;
     for (; v + (BATCH - 1) * THREADS < v1; v += BATCH * THREADS)
     {
         uint4 w[BATCH];
+        float vm[BATCH];
 #pragma unroll
         for (int j = 0; j < BATCH; ++j)
             w[j] = load_vector<TYPE>(row, v + j * THREADS, skew, a.classes);
 #pragma unroll
         for (int j = 0; j < BATCH; ++j)
-            add(w[j], v + j * THREADS);
+            vm[j] = vector_max<TYPE>(w[j]);
+        float most = fmaxf(vm[0], vm[1]);
+#pragma unroll
+        for (int j = 2; j < BATCH; ++j)
+            most = fmaxf(most, vm[j]);
+        if (most > m)
+        {
+            m = most;
+            at = v + (BATCH - 1) * THREADS;
+#pragma unroll
+            for (int j = BATCH - 2; j >= 0; --j)
+                at = vm[j] == most ? v + j * THREADS : at;
+        }
+        if (most > limit)
+            reference(most);
+        if (ordinary)
+        {
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)
+                add(w[j]);
+        }
+        else
+        {
+#pragma unroll 1
+            for (int j = 0; j < BATCH; ++j)
+                add_exactly(j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3]);
+        }
     }
     for (; v < v1; v += THREADS)
-        add(load_vector<TYPE>(row, v, skew, a.classes), v);
-    // relative to the maximum itself
+    {
+        const uint4 w = load_vector<TYPE>(row, v, skew, a.classes);
+        const float vm = vector_max<TYPE>(w);
+        if (vm > m)
+        {
+            m = vm;
+            at = v;
+        }
+        if (vm > limit)
+            reference(vm);
+        if (ordinary)
+            add(w);
+        else
+            add_exactly(w);
+    }
+    // relative to the maximum itself, T in natural units
     float S, T;
     {
         float p, q;
@@ -283,22 +361,26 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, con
         S = p + q;
         halves(T2, p, q);
         T = p + q;
-        const float d = mu - m, c = exp2_approx(d * LOG2E);
         if (m != -INFINITY)
         {
-            T = (T + S * d) * c;
+            const float d = ordinary ? -fmaf(m, LOG2E, -R) : (mu - m) * LOG2E, c = exp2_approx(d);
+            T = (T + S * d) * (c * LN2);
             S *= c;
         }
     }
     const bool any = v0 + tid < v1;
 
     // ---- the CTA's maximum and sums
-    Stats st = {m, S, T};
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1)
+    Stats st;
     {
-        const Stats o = {__shfl_xor_sync(0xffffffffu, st.m, d), __shfl_xor_sync(0xffffffffu, st.S, d), __shfl_xor_sync(0xffffffffu, st.T, d)};
-        st = (lane & d) ? merge(o, st) : merge(st, o);
+        const float wm = value_of(__reduce_max_sync(0xffffffffu, order_of(m)));
+        st = merge({wm, 0.f, 0.f}, {m, S, T}); // its own sums relative to the warp's maximum
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1)
+        {
+            st.S += __shfl_xor_sync(0xffffffffu, st.S, d);
+            st.T += __shfl_xor_sync(0xffffffffu, st.T, d);
+        }
     }
     if (lane == 0)
         sh.part[warp] = st;
@@ -307,57 +389,96 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, con
 
     if (a.top > 0)
     {
-        // ---- the best threads
-        unsigned long long key = sort_lanes<2>(any ? make_key(order_of(m), (uint32_t)at) : 0ull, lane);
-        sh.sorted[warp][lane] = key;
-        for (int step = 1; step < WARPS; step <<= 1)
+        // ---- a bound that at least `top` threads reach: the least of the warps' ceil(top / WARPS) th best keys
+        const unsigned long long key = any ? make_key(order_of(m), (uint32_t)at) : 0ull;
+        unsigned long long nth = 0ull;
         {
-            __syncthreads();
-            if ((warp & (2 * step - 1)) == 0)
+            unsigned long long mine = key;
+            for (int n = 0; n < (a.top + WARPS - 1) / WARPS; ++n)
             {
-                const unsigned long long other = sh.sorted[warp + step][31 - lane];
-                key = sort_lanes<32>(key > other ? key : other, lane);
-                sh.sorted[warp][lane] = key;
+                const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
+                const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32) == high ? (uint32_t)mine : 0u);
+                nth = (unsigned long long)high << 32 | low;
+                mine = mine == nth ? 0ull : mine;
             }
         }
+        if (lane == 0)
+            sh.bound[warp] = nth;
+        if (tid < a.top)
+            sh.best[tid] = 0ull;
+        if (tid == 0)
+            sh.last = 0ull;
+        __syncthreads();
+        unsigned long long bound = sh.bound[0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w)
+            bound = sh.bound[w] < bound ? sh.bound[w] : bound;
+        // ---- those threads, and of them the `top` best
+        if (key != 0ull && key >= bound)
+            sh.found[atomicAdd(&sh.count, 1)] = key;
+        __syncthreads();
+        const int threads = sh.count;
+        if (key != 0ull && key >= bound)
+        {
+            int before = 0;
+            for (int q = 0; q < threads; ++q)
+                before += sh.found[q] > key;
+            if (before < a.top)
+                sh.first[before] = v0 + tid;
+            if (before == a.top - 1)
+                sh.last = key;
+        }
+        __syncthreads();
+        if (tid == 0)
+            sh.count = 0;
         __syncthreads();
         // ---- their elements that are not below the last of them
-        const unsigned long long last = sh.sorted[0][a.top - 1];
+        const int best_threads = min(threads, a.top);
+        const unsigned long long last = sh.last;
         const uint32_t last_order = (uint32_t)(last >> 32), last_vector = 0xffffffffu - (uint32_t)last;
-        const int per_thread = (v1 - v0 + THREADS - 1) / THREADS;
         const bool all = last == 0ull; // fewer threads than that have any
-        auto each = [&](auto take) {
-            for (int i = tid; i < a.top * per_thread; i += THREADS)
+        const float last_value = value_of(last_order); // (not used where `all`)
+        const int per_thread = max(1, (v1 - v0 + THREADS - 1) / THREADS), shift = per_thread > 1 ? 32 - __clz(per_thread - 1) : 0;
+        auto each = [&](auto take) { // all threads over the best threads' vectors, four at a time under way together
+            constexpr int HELD = WARPS == 1 ? 4 : 2;
+            for (int i = tid; i < best_threads << shift; i += HELD * THREADS)
             {
-                const int j = i / per_thread;
-                const unsigned long long k = sh.sorted[0][j];
-                if (k == 0ull)
-                    continue;
-                const int v = v0 + (int)((0xffffffffu - (uint32_t)k - (uint32_t)v0) % THREADS) + (i - j * per_thread) * THREADS;
-                if (v >= v1)
-                    continue;
-                float x[VE];
-                unpack_vector<TYPE>(load_vector<TYPE>(row, v, skew, a.classes), x);
+                uint4 w[HELD];
+                int at[HELD];
 #pragma unroll
-                for (int e = 0; e < VE; ++e)
+                for (int h = 0; h < HELD; ++h)
                 {
-                    const long long index = (long long)v * VE - skew + e;
-                    const uint32_t o = order_of(x[e]);
-                    if (index >= 0 && index < a.classes && (all || o > last_order || (o == last_order && (uint32_t)v <= last_vector)))
-                        take(make_key(o, (uint32_t)index));
+                    const int n = i + h * THREADS;
+                    at[h] = (n >> shift) < best_threads ? sh.first[n >> shift] + (n & ((1 << shift) - 1)) * THREADS : v1;
+                    if (at[h] < v1)
+                        w[h] = load_vector<TYPE>(row, at[h], skew, a.classes);
+                }
+#pragma unroll
+                for (int h = 0; h < HELD; ++h)
+                {
+                    if (at[h] >= v1 || (!all && vector_max<TYPE>(w[h]) < last_value)) // most of them
+                        continue;
+                    float x[VE];
+                    unpack_vector<TYPE>(w[h], x);
+#pragma unroll
+                    for (int e = 0; e < VE; ++e)
+                    {
+                        const long long index = (long long)at[h] * VE - skew + e;
+                        const uint32_t o = order_of(x[e]);
+                        if (index >= 0 && index < a.classes && (all || o > last_order || (o == last_order && (uint32_t)at[h] <= last_vector)))
+                            take(make_key(o, (uint32_t)index));
+                    }
                 }
             }
         };
         each([&](unsigned long long k) {
             const int n = atomicAdd(&sh.count, 1);
-            if (n < CANDIDATES)
+            if (n < ROOM)
                 sh.found[n] = k;
         });
-        if (tid < a.top)
-            sh.best[tid] = 0ull;
         __syncthreads();
         const int n = sh.count;
-        if (n <= CANDIDATES)
+        if (n <= ROOM)
         {
             for (int i = tid; i < n; i += THREADS)
             {
@@ -376,7 +497,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, con
             {
                 unsigned long long k = 0ull;
                 each([&](unsigned long long c) { k = c < limit && c > k ? c : k; });
-                limit = block_max(k, sh.found);
+                limit = block_max<WARPS>(k, sh.found);
                 if (tid == 0)
                     sh.best[j] = limit;
                 if (limit == 0ull)
@@ -388,8 +509,21 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, con
     if (tid == 0)
     {
         Stats s = sh.part[0];
-        for (int w = 1; w < WARPS; ++w)
-            s = merge(s, sh.part[w]);
+        if (WARPS > 1)
+        {
+            float most = s.m;
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w)
+                most = fmaxf(most, sh.part[w].m);
+            s = {most, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) // the same maximum for all, so that no sum waits for the one before it
+            {
+                const Stats o = merge({most, 0.f, 0.f}, sh.part[w]);
+                s.S += o.S;
+                s.T += o.T;
+            }
+        }
         sh.all = s;
     }
 
@@ -440,17 +574,16 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, con
     __syncthreads();
 
     // ---- outputs
-    const Stats s = sh.all;
+    Stats s = sh.all;
+    s.S = max_nan(s.S, 1.f); // the largest class alone gives 1, and what T adds is not positive: roundings apart
+    s.T = s.T > 0.f ? 0.f : s.T;
     const bool nothing = s.m == -INFINITY && !(s.S != s.S); // every class is masked: no probability, no entropy
     const float log_s = nothing ? 0.f : logf(s.S);
     auto logp = [&](float x) { return nothing ? (x != x ? x : -INFINITY) : (x - s.m) - log_s; };
     if (tid == 0)
     {
         if (logprobs)
-        {
-            const long long t = a.token_bytes == 8 ? static_cast<const long long *>(tokens)[r] : static_cast<const int *>(tokens)[r];
-            logprobs[r] = t < 0 ? 0.f : t >= a.classes ? NAN : logp(load1<TYPE>(row, t));
-        }
+            logprobs[r] = token < 0 ? 0.f : token >= a.classes ? NAN : logp(given);
         if (entropy)
             entropy[r] = nothing ? 0.f : log_s - s.T / s.S;
     }
@@ -464,20 +597,20 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpArgs a, con
     }
 }
 
-template <int TYPE>
+template <int TYPE, int WARPS>
 int launch_logprobs(const LogpArgs &a, const void *logits, const void *tokens, float *logprobs, float *entropy, float *top_logprobs,
                     int32_t *top_tokens, cudaStream_t st)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * a.split));
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(32 * WARPS);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)a.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    SB_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<TYPE>, a, logits, tokens, logprobs, entropy, top_logprobs, (int *)top_tokens));
+    SB_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<TYPE, WARPS>, a, logits, tokens, logprobs, entropy, top_logprobs, (int *)top_tokens));
     return launched("logprobs_kernel");
 }
 } // namespace
@@ -511,15 +644,18 @@ extern "C" int small_b200_logprobs(int32_t rows, int32_t classes, int32_t in_typ
     a.rows = rows; a.stride = stride ? stride : classes; a.classes = classes; a.top = top; a.token_bytes = token_bytes;
     // As many CTAs to a row as fill the device twice over, while each of their threads has a vector of its own.
     a.split = 1;
-    while (a.split < MAX_SPLIT && (long long)rows * a.split * 2 <= 2LL * num_sms() && classes / (16 / size) >= 2 * a.split * THREADS)
+    while (a.split < MAX_SPLIT && (long long)rows * a.split * 2 <= 2LL * num_sms() && classes / (16 / size) >= 2 * a.split * 256)
         a.split *= 2;
     if ((long long)rows * a.split > 0x7fffffffLL)
         return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: too many rows.");
     cudaStream_t st = as_stream(stream);
+    const bool narrow = a.split == 1 && classes <= 1024;
+#define SB_LOGP(T, W) launch_logprobs<T, W>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st)
     switch (in_type)
     {
-    case SMALL_B200_TYPE_F32: return launch_logprobs<SMALL_B200_TYPE_F32>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st);
-    case SMALL_B200_TYPE_BF16: return launch_logprobs<SMALL_B200_TYPE_BF16>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st);
-    default: return launch_logprobs<SMALL_B200_TYPE_F16>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st);
+    case SMALL_B200_TYPE_F32: return narrow ? SB_LOGP(SMALL_B200_TYPE_F32, 1) : SB_LOGP(SMALL_B200_TYPE_F32, 8);
+    case SMALL_B200_TYPE_BF16: return narrow ? SB_LOGP(SMALL_B200_TYPE_BF16, 1) : SB_LOGP(SMALL_B200_TYPE_BF16, 8);
+    default: return narrow ? SB_LOGP(SMALL_B200_TYPE_F16, 1) : SB_LOGP(SMALL_B200_TYPE_F16, 8);
     }
+#undef SB_LOGP
 }
