@@ -5,9 +5,10 @@
 // Every thread keeps (m, S, T) of the vectors it has read and rescales when its maximum has moved far; pairs merge as S = sum S_j e^(m_j - m),
 // T = sum (T_j + S_j (m_j - m)) e^(m_j - m).  A masked class (minus infinity, or a value so low that its exponential is 0) adds 0 to both.
 //
-// Best alternatives: a thread also remembers which of its vectors first held its maximum.  These (value, vector) keys are all different, and the
-// `top` best elements lie in the `top` threads with the best keys: an element elsewhere has those threads' maxima before it.  Only these
-// threads' vectors are read again (from L2), and only elements not below the last of the keys are ranked.
+// Best alternatives: for each quarter of its vectors a thread also remembers the maximum and which of them first held it.  These (value, vector) keys are all
+// different, and the `top` best elements lie in the `top` parts with the best keys: an element elsewhere has those parts' maxima before it.
+// Only these parts' vectors are read again, and only elements not below the last of the keys are ranked.  (Rows are read by so many CTAs at once that L2
+// does not hold them: with whole threads in place of quarters the second reading of 8 of 256 threads took 14 us of 107 at 2048 rows of 131072 classes.)
 //
 // Bound: memory, every logit read once.  A row is cut among the CTAs of a cluster where rows are few, and what they found is merged over distributed
 // shared memory: no workspace, and sums are always added in the same order.
@@ -21,7 +22,7 @@ namespace
 using namespace sb;
 
 constexpr int TOP_MOST = 32, MAX_SPLIT = 8;
-constexpr int CANDIDATES = 1024;
+constexpr int CANDIDATES = 1024, PARTS = 4;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f, SLACK = 4.f;
 
 struct LogpArgs
@@ -193,6 +194,15 @@ struct Masked
     }
 };
 
+// The barrier of a row's threads.
+template <int WARPS>
+__device__ __forceinline__ void sync_row()
+{
+    if (WARPS == 1)
+        __syncwarp();
+    else
+        __syncthreads();
+}
 template <int WARPS>
 __device__ __forceinline__ unsigned long long block_max(unsigned long long key, unsigned long long *part)
 {
@@ -202,10 +212,10 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long key, 
         const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, d);
         key = key > other ? key : other;
     }
-    __syncthreads();
+    sync_row<WARPS>();
     if ((threadIdx.x & 31) == 0)
-        part[threadIdx.x >> 5] = key;
-    __syncthreads();
+        part[WARPS == 1 ? 0 : threadIdx.x >> 5] = key;
+    sync_row<WARPS>();
     key = part[0];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w)
@@ -220,21 +230,26 @@ struct Shared
     unsigned long long bound[WARPS], last;
     unsigned long long best[TOP_MOST]; // this CTA's best elements, in order
     unsigned long long found[WARPS == 1 ? 256 : CANDIDATES];
+    unsigned long long keys[PARTS * 32 * WARPS];
     unsigned long long merged[WARPS == 1 ? 1 : MAX_SPLIT * TOP_MOST];
     int first[TOP_MOST]; // the best threads' first vectors
     int count;
 };
 
 template <int TYPE, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens,
+__global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_F32 ? 4 : 5) logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens,
                                                             float *__restrict__ logprobs, float *__restrict__ entropy,
                                                             float *__restrict__ top_logprobs, int *__restrict__ top_tokens)
 {
     constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, BATCH = 4, THREADS = 32 * WARPS;
     constexpr int ROOM = sizeof(Shared<WARPS>::found) / 8;
-    __shared__ Shared<WARPS> sh;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long r = blockIdx.x / a.split;
+    constexpr int ROWS = 8 / WARPS; // of a CTA
+    __shared__ Shared<WARPS> of_row[ROWS];
+    Shared<WARPS> &sh = of_row[WARPS == 1 ? threadIdx.x >> 5 : 0];
+    const int tid = threadIdx.x & (THREADS - 1), lane = tid & 31, warp = tid >> 5;
+    const long long r = WARPS == 1 ? (long long)blockIdx.x * ROWS + (threadIdx.x >> 5) : blockIdx.x / a.split;
+    if (r >= a.rows)
+        return;
     const int rank = (int)(blockIdx.x % a.split);
     const char *row = static_cast<const char *>(logits) + r * a.stride * SIZE;
     const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / SIZE);
@@ -258,7 +273,10 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
     bool ordinary = true;
     unsigned long long S2 = 0ull, T2 = 0ull, minus_R = 0ull;
     const unsigned long long log2e2 = pair(LOG2E, LOG2E);
-    int at = v0 + tid; // the vector that held m first
+    // The best elements are looked for in the parts whose maxima are the largest: a thread's vectors in PARTS parts, `part` steps each.  key[q]: the part's
+    // maximum and the vector that held it first, 0 without any.
+    const int part = max(1, ((v1 - v0 + THREADS - 1) / THREADS + PARTS * BATCH - 1) / (PARTS * BATCH));
+    unsigned long long *keys = sh.keys + tid;
     auto reference = [&](float vm) {
         const bool now = vm > Masked<TYPE>::ORDINARY && vm < 1e6f;
         const float to = vm * LOG2E;
@@ -299,59 +317,71 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
             T2 = fma2(e, pair(p, q), T2);
         }
     };
+    const uint4 *aligned = reinterpret_cast<const uint4 *>(row - skew * SIZE);
+    const int whole0 = skew > 0 ? 1 : 0, whole1 = min(v1, (int)(((long long)skew + a.classes) / VE)); // vectors with elements of this row only
     int v = v0 + tid;
-    for (; v + (BATCH - 1) * THREADS < v1; v += BATCH * THREADS)
-    {
-        uint4 w[BATCH];
-        float vm[BATCH];
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j)
-            w[j] = load_vector<TYPE>(row, v + j * THREADS, skew, a.classes);
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j)
-            vm[j] = vector_max<TYPE>(w[j]);
-        float most = fmaxf(vm[0], vm[1]);
-#pragma unroll
-        for (int j = 2; j < BATCH; ++j)
-            most = fmaxf(most, vm[j]);
-        if (most > m)
-        {
-            m = most;
-            at = v + (BATCH - 1) * THREADS;
-#pragma unroll
-            for (int j = BATCH - 2; j >= 0; --j)
-                at = vm[j] == most ? v + j * THREADS : at;
-        }
-        if (most > limit)
-            reference(most);
-        if (ordinary)
-        {
-#pragma unroll
-            for (int j = 0; j < BATCH; ++j)
-                add(w[j]);
-        }
-        else
-        {
 #pragma unroll 1
-            for (int j = 0; j < BATCH; ++j)
-                add_exactly(j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3]);
-        }
-    }
-    for (; v < v1; v += THREADS)
+    for (int q = 0; q < PARTS; ++q)
     {
-        const uint4 w = load_vector<TYPE>(row, v, skew, a.classes);
-        const float vm = vector_max<TYPE>(w);
-        if (vm > m)
+        const int end = (int)min((long long)v1, v0 + (q + 1LL) * part * BATCH * THREADS), whole = min(end, whole1), begin = v;
+        float pm = -INFINITY;
+        int at = v;
+        for (; v + (BATCH - 1) * THREADS < whole; v += BATCH * THREADS)
         {
-            m = vm;
-            at = v;
+            uint4 w[BATCH];
+            float vm[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)
+                w[j] = j == 0 && v < whole0 ? load_vector<TYPE>(row, v, skew, a.classes) : __ldg(aligned + v + j * THREADS);
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)
+                vm[j] = vector_max<TYPE>(w[j]);
+            float most = fmaxf(vm[0], vm[1]);
+#pragma unroll
+            for (int j = 2; j < BATCH; ++j)
+                most = fmaxf(most, vm[j]);
+            if (most > pm)
+            {
+                pm = most;
+                at = v + (BATCH - 1) * THREADS;
+#pragma unroll
+                for (int j = BATCH - 2; j >= 0; --j)
+                    at = vm[j] == most ? v + j * THREADS : at;
+            }
+            if (most > limit)
+                reference(most);
+            if (ordinary)
+            {
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j)
+                    add(w[j]);
+            }
+            else
+            {
+#pragma unroll 1
+                for (int j = 0; j < BATCH; ++j)
+                    add_exactly(j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3]);
+            }
         }
-        if (vm > limit)
-            reference(vm);
-        if (ordinary)
-            add(w);
-        else
-            add_exactly(w);
+#pragma unroll 1
+        for (; v < end; v += THREADS)
+        {
+            const uint4 w = load_vector<TYPE>(row, v, skew, a.classes);
+            const float vm = vector_max<TYPE>(w);
+            if (vm > pm)
+            {
+                pm = vm;
+                at = v;
+            }
+            if (vm > limit)
+                reference(vm);
+            if (ordinary)
+                add(w);
+            else
+                add_exactly(w);
+        }
+        keys[q * THREADS] = begin < end ? make_key(order_of(pm), (uint32_t)at) : 0ull;
+        m = fmaxf(m, pm);
     }
     // relative to the maximum itself, T in natural units
     float S, T;
@@ -368,7 +398,6 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
             S *= c;
         }
     }
-    const bool any = v0 + tid < v1;
 
     // ---- the CTA's maximum and sums
     Stats st;
@@ -389,11 +418,17 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
 
     if (a.top > 0)
     {
-        // ---- a bound that at least `top` threads reach: the least of the warps' ceil(top / WARPS) th best keys
-        const unsigned long long key = any ? make_key(order_of(m), (uint32_t)at) : 0ull;
+        // ---- a bound that at least `top` parts reach: the least of the warps' ceil(top / WARPS) th best keys of their threads
+        unsigned long long key[PARTS], most = 0ull;
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+        {
+            key[q] = keys[q * THREADS];
+            most = key[q] > most ? key[q] : most;
+        }
         unsigned long long nth = 0ull;
         {
-            unsigned long long mine = key;
+            unsigned long long mine = most;
             for (int n = 0; n < (a.top + WARPS - 1) / WARPS; ++n)
             {
                 const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
@@ -408,40 +443,47 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
             sh.best[tid] = 0ull;
         if (tid == 0)
             sh.last = 0ull;
-        __syncthreads();
+        sync_row<WARPS>();
         unsigned long long bound = sh.bound[0];
 #pragma unroll
         for (int w = 1; w < WARPS; ++w)
             bound = sh.bound[w] < bound ? sh.bound[w] : bound;
-        // ---- those threads, and of them the `top` best
-        if (key != 0ull && key >= bound)
-            sh.found[atomicAdd(&sh.count, 1)] = key;
-        __syncthreads();
-        const int threads = sh.count;
-        if (key != 0ull && key >= bound)
+        // ---- the parts that reach it, and of them the `top` best
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+            if (key[q] != 0ull && key[q] >= bound)
+                sh.found[atomicAdd(&sh.count, 1)] = key[q];
+        sync_row<WARPS>();
+        const int reach = sh.count;
+        for (int i = tid; i < reach; i += THREADS)
         {
+            const unsigned long long k = sh.found[i];
             int before = 0;
-            for (int q = 0; q < threads; ++q)
-                before += sh.found[q] > key;
+#pragma unroll 4
+            for (int q = 0; q < reach; ++q)
+                before += sh.found[q] > k;
             if (before < a.top)
-                sh.first[before] = v0 + tid;
+            {
+                const int steps_in = (int)(0xffffffffu - (uint32_t)k - (uint32_t)v0) / THREADS, thread = (int)(0xffffffffu - (uint32_t)k - (uint32_t)v0) % THREADS;
+                sh.first[before] = v0 + thread + steps_in / (part * BATCH) * (part * BATCH) * THREADS;
+            }
             if (before == a.top - 1)
-                sh.last = key;
+                sh.last = k;
         }
-        __syncthreads();
+        sync_row<WARPS>();
         if (tid == 0)
             sh.count = 0;
-        __syncthreads();
+        sync_row<WARPS>();
         // ---- their elements that are not below the last of them
-        const int best_threads = min(threads, a.top);
+        const int best_parts = min(reach, a.top);
         const unsigned long long last = sh.last;
         const uint32_t last_order = (uint32_t)(last >> 32), last_vector = 0xffffffffu - (uint32_t)last;
         const bool all = last == 0ull; // fewer threads than that have any
         const float last_value = value_of(last_order); // (not used where `all`)
-        const int per_thread = max(1, (v1 - v0 + THREADS - 1) / THREADS), shift = per_thread > 1 ? 32 - __clz(per_thread - 1) : 0;
+        const int in_part = part * BATCH, shift = 32 - __clz(in_part - 1); // (four vectors at least)
         auto each = [&](auto take) { // all threads over the best threads' vectors, four at a time under way together
             constexpr int HELD = WARPS == 1 ? 4 : 2;
-            for (int i = tid; i < best_threads << shift; i += HELD * THREADS)
+            for (int i = tid; i < best_parts << shift; i += HELD * THREADS)
             {
                 uint4 w[HELD];
                 int at[HELD];
@@ -449,7 +491,8 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
                 for (int h = 0; h < HELD; ++h)
                 {
                     const int n = i + h * THREADS;
-                    at[h] = (n >> shift) < best_threads ? sh.first[n >> shift] + (n & ((1 << shift) - 1)) * THREADS : v1;
+                    const int i_in = n & ((1 << shift) - 1);
+                    at[h] = (n >> shift) < best_parts && i_in < in_part ? sh.first[n >> shift] + i_in * THREADS : v1;
                     if (at[h] < v1)
                         w[h] = load_vector<TYPE>(row, at[h], skew, a.classes);
                 }
@@ -476,7 +519,7 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
             if (n < ROOM)
                 sh.found[n] = k;
         });
-        __syncthreads();
+        sync_row<WARPS>();
         const int n = sh.count;
         if (n <= ROOM)
         {
@@ -484,6 +527,7 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
             {
                 const unsigned long long k = sh.found[i];
                 int before = 0;
+#pragma unroll 4
                 for (int q = 0; q < n; ++q)
                     before += sh.found[q] > k;
                 if (before < a.top)
@@ -505,7 +549,7 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
             }
         }
     }
-    __syncthreads();
+    sync_row<WARPS>();
     if (tid == 0)
     {
         Stats s = sh.part[0];
@@ -555,7 +599,7 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
                 asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(map_to_cta(&sh.best[i % a.top], i / a.top)));
                 sh.merged[i] = k;
             }
-            __syncthreads();
+            sync_row<WARPS>();
             for (int i = tid; i < n; i += THREADS)
             {
                 const unsigned long long k = sh.merged[i];
@@ -571,7 +615,7 @@ __global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(const LogpArgs a, 
         if (rank != 0)
             return;
     }
-    __syncthreads();
+    sync_row<WARPS>();
 
     // ---- outputs
     Stats s = sh.all;
@@ -602,8 +646,8 @@ int launch_logprobs(const LogpArgs &a, const void *logits, const void *tokens, f
                     int32_t *top_tokens, cudaStream_t st)
 {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.rows * a.split));
-    cfg.blockDim = dim3(32 * WARPS);
+    cfg.gridDim = dim3((unsigned)(WARPS == 1 ? (a.rows + 7) / 8 : a.rows * a.split));
+    cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -642,9 +686,9 @@ extern "C" int small_b200_logprobs(int32_t rows, int32_t classes, int32_t in_typ
         return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: misaligned buffer.");
     LogpArgs a;
     a.rows = rows; a.stride = stride ? stride : classes; a.classes = classes; a.top = top; a.token_bytes = token_bytes;
-    // As many CTAs to a row as fill the device twice over, while each of their threads has a vector of its own.
+    // As many CTAs to a row as are resident at once, while each of their threads has a vector of its own.
     a.split = 1;
-    while (a.split < MAX_SPLIT && (long long)rows * a.split * 2 <= 2LL * num_sms() && classes / (16 / size) >= 2 * a.split * 256)
+    while (a.split < MAX_SPLIT && (long long)rows * a.split * 2 <= 4LL * num_sms() && classes / (16 / size) >= 2 * a.split * 256)
         a.split *= 2;
     if ((long long)rows * a.split > 0x7fffffffLL)
         return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: too many rows.");
