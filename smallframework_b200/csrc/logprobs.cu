@@ -11,7 +11,7 @@
 // does not hold them: with whole threads in place of quarters the second reading of 8 of 256 threads took 14 us of 107 at 2048 rows of 131072 classes.)
 //
 // Bound: memory, every logit read once.  A row is cut among the CTAs of a cluster where rows are few, and what they found is merged over distributed
-// shared memory: no workspace, and sums are always added in the same order.
+// shared memory (asynchronous stores to the first CTA): no workspace, and sums are always added in the same order.
 #include <algorithm>
 
 #include "narrow_types.cuh"
@@ -232,14 +232,16 @@ struct Shared
     unsigned long long found[WARPS == 1 ? 256 : CANDIDATES];
     unsigned long long keys[PARTS * 32 * WARPS];
     unsigned long long merged[WARPS == 1 ? 1 : MAX_SPLIT * TOP_MOST];
-    int first[TOP_MOST]; // the best threads' first vectors
+    float4 of_cta[MAX_SPLIT]; // every CTA's maximum and sums, in the first
+    int first[TOP_MOST];      // the best parts' first vectors
     int count;
+    uint64_t delivered;
 };
 
 template <int TYPE, int WARPS>
 __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_F32 ? 4 : 5) logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens,
                                                             float *__restrict__ logprobs, float *__restrict__ entropy,
-                                                            float *__restrict__ top_logprobs, int *__restrict__ top_tokens)
+                                                            float *__restrict__ top_logprobs, int *__restrict__ top_tokens, int *status)
 {
     constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, BATCH = 4, THREADS = 32 * WARPS;
     constexpr int ROOM = sizeof(Shared<WARPS>::found) / 8;
@@ -256,6 +258,17 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
     const int vectors = (int)(((long long)skew + a.classes + VE - 1) / VE);
     const int share = (vectors + a.split - 1) / a.split;
     const int v0 = rank * share, v1 = min(vectors, v0 + share);
+    if (WARPS > 1 && a.split > 1)
+    {
+        if (tid == 0)
+        {
+            mbar_init(&sh.delivered, 1);
+            fence_barrier_init();
+            mbar_expect_tx(&sh.delivered, (uint32_t)(a.split * (8 * a.top + 16)));
+        }
+        __syncwarp();
+        cluster_arrive_release();
+    }
     // the given class's logit, asked for before everything else
     long long token = -1;
     float given = 0.f;
@@ -571,39 +584,47 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
         sh.all = s;
     }
 
-    // ---- the cluster's, in the first CTA
+    // ---- the cluster's, in the first CTA: the others send it what they have
     const unsigned long long *best = sh.best;
-    if (a.split > 1)
+    sync_row<WARPS>();
+    if (WARPS > 1 && a.split > 1)
     {
-        cluster_sync_all();
+        cluster_wait(); // the first CTA's barrier is there
+        const uint32_t bar = map_to_cta(&sh.delivered, 0);
+        if (tid < a.top)
+            st_async_b64(map_to_cta(&sh.merged[rank * a.top + tid], 0), sh.best[tid], bar);
+        if (tid == 32)
+        {
+            const uint32_t to = map_to_cta(&sh.of_cta[rank], 0);
+            st_async_b64(to, pair(sh.all.m, sh.all.S), bar);
+            st_async_b64(to + 8, pair(sh.all.T, 0.f), bar);
+        }
+        __syncwarp();
+        cluster_arrive_relaxed(); // nothing more is sent
+        bool delivered = true;
         if (rank == 0)
         {
+            delivered = mbar_wait_cluster(&sh.delivered, 0, status, 121);
             if (tid == 0)
             {
-                Stats s = sh.all;
+                float most = sh.of_cta[0].x;
                 for (int q = 1; q < a.split; ++q)
+                    most = fmaxf(most, sh.of_cta[q].x);
+                Stats s = {most, 0.f, 0.f};
+                for (int q = 0; q < a.split; ++q)
                 {
-                    const uint32_t p = map_to_cta(&sh.all, q);
-                    Stats o;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.m) : "r"(p));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1+4];" : "=f"(o.S) : "r"(p));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1+8];" : "=f"(o.T) : "r"(p));
-                    s = merge(s, o);
+                    const Stats o = merge({most, 0.f, 0.f}, {sh.of_cta[q].x, sh.of_cta[q].y, sh.of_cta[q].z});
+                    s.S += o.S;
+                    s.T += o.T;
                 }
                 sh.all = s;
             }
             const int n = a.split * a.top;
             for (int i = tid; i < n; i += THREADS)
             {
-                unsigned long long k;
-                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(map_to_cta(&sh.best[i % a.top], i / a.top)));
-                sh.merged[i] = k;
-            }
-            sync_row<WARPS>();
-            for (int i = tid; i < n; i += THREADS)
-            {
                 const unsigned long long k = sh.merged[i];
                 int before = 0;
+#pragma unroll 4
                 for (int q = 0; q < n; ++q)
                     before += sh.merged[q] > k;
                 if (k != 0ull && before < a.top)
@@ -611,11 +632,14 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
             }
             best = sh.found;
         }
-        cluster_sync_all(); // nobody's shared memory goes while it is read
+        cluster_wait(); // the first CTA's shared memory stays while anybody may send to it
+        if (!delivered)
+            for (int i = 0; i < 1000; ++i)
+                __nanosleep(1000); // and what was sent last is on its way for less than that
         if (rank != 0)
             return;
+        sync_row<WARPS>();
     }
-    sync_row<WARPS>();
 
     // ---- outputs
     Stats s = sh.all;
@@ -645,6 +669,9 @@ template <int TYPE, int WARPS>
 int launch_logprobs(const LogpArgs &a, const void *logits, const void *tokens, float *logprobs, float *entropy, float *top_logprobs,
                     int32_t *top_tokens, cudaStream_t st)
 {
+    int *status = device_status_ptr();
+    if (!status)
+        return fail(SMALL_B200_CUDA_ERROR, "device status word not available");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(WARPS == 1 ? (a.rows + 7) / 8 : a.rows * a.split));
     cfg.blockDim = dim3(256);
@@ -654,7 +681,7 @@ int launch_logprobs(const LogpArgs &a, const void *logits, const void *tokens, f
     attr[0].val.clusterDim.x = (unsigned)a.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    SB_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<TYPE, WARPS>, a, logits, tokens, logprobs, entropy, top_logprobs, (int *)top_tokens));
+    SB_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<TYPE, WARPS>, a, logits, tokens, logprobs, entropy, top_logprobs, (int *)top_tokens, status));
     return launched("logprobs_kernel");
 }
 } // namespace
