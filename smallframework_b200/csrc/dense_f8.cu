@@ -130,16 +130,19 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
         tma_load_2d(ring + s * G::STAGE + A_BYTES, &map_x, (b0 + i) * KB, r0, &full[s]);
     };
 
+    // The loading warp does not wait for the others, nor they for it: under load it takes microseconds until the last of its first copies is accepted.
     if (warp == 4)
     {
-        // the first stages are on their way before anything else is set up
         if (elect_one())
         {
             for (int s = 0; s < G::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
             fence_barrier_init();
+        }
+        __syncwarp();
+        asm volatile("bar.arrive 1, %0;" ::"n"(FEW_THREADS) : "memory");
+        if (elect_one())
             for (int i = 0; i < G::STAGES && i < n; ++i)
                 load(i, i);
-        }
         __syncwarp();
     }
     else if (warp == 5)
@@ -156,11 +159,13 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
         fence_barrier_init();
         mbar_expect_tx(&delivered, G::INBOX);
     }
-    // ---- scales: the product of a row's and the weights' scale, by block and row; the first ones are asked for here
+    // ---- scales: the product of a row's and the weights' scale, by block and row
     constexpr int ROWS = (BN + 31) / 32;
-    float sv[ROWS][G::CHUNK];
+    float sv[ROWS][G::CHUNK], sw[G::CHUNK]; // multiplied when they are needed: until then nothing waits for them
     auto ask = [&](int c) {
-        const float *sw = a.filt_scales + (size_t)kt * a.blocks + b0;
+#pragma unroll
+        for (int j = 0; j < G::CHUNK; ++j)
+            sw[j] = c * G::CHUNK + j < n ? __ldg(a.filt_scales + (size_t)kt * a.blocks + b0 + c * G::CHUNK + j) : 0.f;
 #pragma unroll
         for (int q = 0; q < ROWS; ++q)
         {
@@ -170,15 +175,15 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
             for (int j = 0; j < G::CHUNK; ++j)
             {
                 const int b = c * G::CHUNK + j;
-                sv[q][j] = col < BN && row < a.rows && b < n ? __ldg(sx + b) * __ldg(sw + b) : 0.f;
+                sv[q][j] = col < BN && row < a.rows && b < n ? __ldg(sx + b) : 0.f;
             }
         }
     };
-    if (warp == 6)
-        ask(0);
     tc_fence_before_sync();
-    __syncthreads();
-    cluster_arrive_release(); // this CTA's inbox can be written to
+    if (warp != 4)
+        asm volatile("bar.sync 1, %0;" ::"n"(FEW_THREADS) : "memory");
+    __syncwarp();
+    cluster_arrive_relaxed(); // this CTA's inbox can be written to: its barrier has been made and fenced
     tc_fence_after_sync();
     const uint32_t tmem = tmem_s;
     unsigned long long acc[BN / 2]; // of the folding warps
@@ -305,8 +310,7 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
         const int chunks = (n + G::CHUNK - 1) / G::CHUNK;
         for (int c = 0; c < chunks; ++c)
         {
-            if (c > 0)
-                ask(c);
+            ask(c);
             const bool ok = c < 2 || mbar_wait(&sc_empty[c & 1], ((c >> 1) - 1) & 1, status, 108);
             if (!__all_sync(0xffffffffu, ok))
                 break;
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
 #pragma unroll
                 for (int j = 0; j < G::CHUNK; ++j)
                     if (q * 32 + lane < BN)
-                        scales[((c & 1) * G::CHUNK + j) * BN + q * 32 + lane] = sv[q][j];
+                        scales[((c & 1) * G::CHUNK + j) * BN + q * 32 + lane] = sv[q][j] * sw[j];
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(&sc_full[c & 1]);
@@ -323,21 +327,37 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
     }
     __syncwarp();
 
+    // tensor memory has been read
+    tc_fence_before_sync();
+    if (warp < 4)
+        asm volatile("bar.arrive 2, 160;" ::: "memory");
+    else if (warp == 5)
+    {
+        asm volatile("bar.sync 2, 160;" ::: "memory");
+        tmem_dealloc(tmem, G::COLS);
+    }
+    __syncwarp();
     // ---- every CTA of the cluster has a share of the rows: the others send it what they have of them (a wait that gave up leaves rubbish, which
     // the status word tells)
     cluster_wait(); // all inboxes can be written to
     const int per = BN / a.split;
     if (warp < 4)
     {
-        int to = 0, pair = 0; // c = to * per + 2 * pair
+        const unsigned long long *mine = inbox + rank * (per / 2) * 128 + tid;
+        int to = 0, left = per; // of the share that is being sent
+        uint32_t at = map_to_cta(mine, 0), bar = map_to_cta(&delivered, 0);
 #pragma unroll
         for (int c = 0; c < BN; c += 2)
         {
-            st_async_b64(map_to_cta(inbox + (rank * (per / 2) + pair) * 128 + tid, to), acc[c / 2], map_to_cta(&delivered, to));
-            if (2 * ++pair == per)
+            st_async_b64(at, acc[c / 2], bar);
+            at += 128 * 8;
+            left -= 2;
+            if (left == 0 && c + 2 < BN)
             {
-                pair = 0;
+                left = per;
                 ++to;
+                at = map_to_cta(mine, to);
+                bar = map_to_cta(&delivered, to);
             }
         }
     }
@@ -367,10 +387,6 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
     if (!all)
         for (int i = 0; i < 1000; ++i)
             __nanosleep(1000); // and what was sent last is on its way for less than that
-    tc_fence_before_sync();
-    __syncthreads();
-    if (warp == 5)
-        tmem_dealloc(tmem, G::COLS);
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -424,7 +440,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
         tmem_alloc_pair(&tmem_s, 512);
     tc_fence_before_sync();
     __syncthreads();
-    cluster_sync_all();
+    cluster_arrive_relaxed(); // the barriers have been made and fenced
+    cluster_wait();
     tc_fence_after_sync();
     const uint32_t tmem = tmem_s;
 
@@ -721,9 +738,10 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
         const int bn = D->rows <= 16 ? 16 : D->rows <= 32 ? 32 : 64;
         a.k_tiles = (D->K + 127) / 128;
         a.r_tiles = (D->rows + bn - 1) / bn;
-        // Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each at least two blocks.
+        // Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each at least two blocks.  Clusters of eight come up slowly
+        // (the last of 32 after 1.8 us, of 64 clusters of four after 0.9): only where four leave SMs without a CTA.
         a.split = 1;
-        while (a.split < 8 && (long long)a.k_tiles * a.r_tiles * a.split * 2 <= 2LL * num_sms() && a.blocks >= 4 * a.split)
+        while (a.split < 8 && (long long)a.k_tiles * a.r_tiles * a.split * 2 <= (a.split < 4 ? 2LL : 1LL) * num_sms() && a.blocks >= 4 * a.split)
             a.split *= 2;
         if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, 128))
             return rc;

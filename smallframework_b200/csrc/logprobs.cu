@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
             mbar_expect_tx(&sh.delivered, (uint32_t)(a.split * (8 * a.top + 16)));
         }
         __syncwarp();
-        cluster_arrive_release();
+        cluster_arrive_relaxed();
     }
     // the given class's logit, asked for before everything else
     long long token = -1;

@@ -138,12 +138,8 @@ __device__ __forceinline__ void cluster_sync_all()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The barrier's two halves, for work in between.  Every thread of the cluster arrives and waits; a relaxed arrival says no more than that this thread has come
-// this far (a release waits until its stores to global memory are performed, a microsecond).
-__device__ __forceinline__ void cluster_arrive_release()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
+// The barrier's two halves, for work in between.  Every thread of the cluster arrives and waits; the arrival says no more than that this thread has come
+// this far, which is enough for barriers that have been made and fenced (a release costs half a microsecond, and a whole one behind stores to global memory).
 __device__ __forceinline__ void cluster_arrive_relaxed()
 {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");

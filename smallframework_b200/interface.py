@@ -687,7 +687,7 @@ def _size(name, n):
         raise ValueError(f"{name}: a size of {n}")
 
 
-_F32, _F8, _TOKENS, _I32 = (torch.float32,), (torch.float8_e4m3fn,), (torch.int32, torch.int64), (torch.int32,)
+_F32, _F8, _I32, _TOKENS = torch.float32, torch.float8_e4m3fn, torch.int32, (torch.int32, torch.int64)
 _FLOATS = tuple(_TYPES)
 
 
@@ -705,10 +705,17 @@ def QuantizeBlocks(num_rows, num_columns, input_buf, output_buf, *, input_stride
     apart = num_columns if input_stride is None else input_stride
     x = _tensor(input_buf)
     here = _home(name, x, "input")
-    at = _at(name, x, (num_rows - 1) * apart + num_columns if num_rows > 0 else 0, "input", _FLOATS, here)
-    check(lib().small_b200_quantize_blocks_f8(num_rows, num_columns, output_buf.block_rows, _TYPES[x.dtype], at, apart,
-                                              _at(name, output_buf.t, num_rows * num_columns, "output", _F8, here),
-                                              _at(name, output_buf.scales, -(-num_rows // output_buf.block_rows) * -(-num_columns // 128), "scales", _F32, here), _stream(stream)))
+    q, scales, m = output_buf.t, output_buf.scales, output_buf.block_rows
+    elems, n = (num_rows - 1) * apart + num_columns if num_rows > 0 else 0, -(-num_rows // m) * -(-num_columns // 128)
+    # all of it in one expression: a call to _at for each tensor takes 0.2 us more
+    if not (x.dtype in _TYPES and x.numel() >= elems and x.is_contiguous()
+            and q.get_device() == here and q.dtype is _F8 and q.numel() >= num_rows * num_columns and q.is_contiguous()
+            and scales.get_device() == here and scales.dtype is _F32 and scales.numel() >= n and scales.is_contiguous()):
+        _at(name, x, elems, "input", _FLOATS, here)
+        _at(name, q, num_rows * num_columns, "output", (_F8,), here)
+        _at(name, scales, n, "scales", (_F32,), here)
+    check(lib().small_b200_quantize_blocks_f8(num_rows, num_columns, m, _TYPES[x.dtype], x.data_ptr(), apart, q.data_ptr(), scales.data_ptr(),
+                                              _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)))
 
 
 def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, out_stride, stream):
@@ -727,10 +734,21 @@ def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, o
     apart = K if out_stride is None else out_stride
     L = _dense_layer(rows, K, C_, _TYPES[y.dtype], apart, accumulate, act, slope)
     blocks, here = -(-C_ // 128), _home(name, y, "output")
-    check(lib().small_b200_dense_f8(L, _at(name, inp.t, rows * C_, "input", _F8, here), _at(name, inp.scales, rows * blocks, "input scales", _F32, here),
-                                    _at(name, filt.t, K * C_, "filter", _F8, here), _at(name, filt.scales, -(-K // 128) * blocks, "filter scales", _F32, here),
-                                    None if bias is None else _at(name, _tensor(bias), K, "bias", _F32, here),
-                                    _at(name, y, (rows - 1) * apart + K if rows > 0 else 0, "output", _FLOATS, here), _stream(stream)))
+    elems = (rows - 1) * apart + K if rows > 0 else 0
+    x, xs, w, ws = inp.t, inp.scales, filt.t, filt.scales
+    if not (y.numel() >= elems and y.is_contiguous()
+            and x.get_device() == here and x.dtype is _F8 and x.numel() >= rows * C_ and x.is_contiguous()
+            and xs.get_device() == here and xs.dtype is _F32 and xs.numel() >= rows * blocks and xs.is_contiguous()
+            and w.get_device() == here and w.dtype is _F8 and w.numel() >= K * C_ and w.is_contiguous()
+            and ws.get_device() == here and ws.dtype is _F32 and ws.numel() >= -(-K // 128) * blocks and ws.is_contiguous()):
+        _at(name, y, elems, "output", _FLOATS, here)
+        _at(name, x, rows * C_, "input", (_F8,), here)
+        _at(name, xs, rows * blocks, "input scales", (_F32,), here)
+        _at(name, w, K * C_, "filter", (_F8,), here)
+        _at(name, ws, -(-K // 128) * blocks, "filter scales", (_F32,), here)
+    check(lib().small_b200_dense_f8(L, x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(),
+                                    None if bias is None else _at(name, _tensor(bias), K, "bias", (_F32,), here), y.data_ptr(),
+                                    _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -756,15 +774,36 @@ def LogProbabilities(num_rows, num_classes, logits_buf, tokens, logprobs_buf, en
     apart = num_classes if row_stride is None else row_stride
     x = _tensor(logits_buf)
     here = _home(name, x, "logits")
-    at = _at(name, x, (num_rows - 1) * apart + num_classes if num_rows > 0 else 0, "logits", _FLOATS, here)
-    each = num_rows * top
-    check(lib().small_b200_logprobs(
-        num_rows, num_classes, _TYPES[x.dtype], at, apart, 4 if tokens is None else tokens.element_size(),
-        None if tokens is None else _at(name, tokens, num_rows, "tokens", _TOKENS, here),
-        None if logprobs_buf is None else _at(name, _tensor(logprobs_buf), num_rows, "log-probabilities", _F32, here),
-        None if entropy_buf is None else _at(name, _tensor(entropy_buf), num_rows, "entropy", _F32, here), top,
-        None if top_logprobs_buf is None else _at(name, _tensor(top_logprobs_buf), each, "top log-probabilities", _F32, here),
-        None if top_tokens is None else _at(name, top_tokens, each, "top tokens", _I32, here), _stream(stream)))
+    elems, each = (num_rows - 1) * apart + num_classes if num_rows > 0 else 0, num_rows * top
+    if not (x.dtype in _TYPES and x.numel() >= elems and x.is_contiguous()):
+        _at(name, x, elems, "logits", _FLOATS, here)
+    given = lp = h = tv = ti = None
+    wide = 4
+    if tokens is not None:
+        if not (tokens.get_device() == here and tokens.dtype in _TOKENS and tokens.numel() >= num_rows and tokens.is_contiguous()):
+            _at(name, tokens, num_rows, "tokens", _TOKENS, here)
+        given, wide = tokens.data_ptr(), tokens.element_size()
+    if logprobs_buf is not None:
+        t = logprobs_buf if isinstance(logprobs_buf, torch.Tensor) else logprobs_buf.t
+        if not (t.get_device() == here and t.dtype is _F32 and t.numel() >= num_rows and t.is_contiguous()):
+            _at(name, t, num_rows, "log-probabilities", (_F32,), here)
+        lp = t.data_ptr()
+    if entropy_buf is not None:
+        t = entropy_buf if isinstance(entropy_buf, torch.Tensor) else entropy_buf.t
+        if not (t.get_device() == here and t.dtype is _F32 and t.numel() >= num_rows and t.is_contiguous()):
+            _at(name, t, num_rows, "entropy", (_F32,), here)
+        h = t.data_ptr()
+    if top_logprobs_buf is not None:
+        t = top_logprobs_buf if isinstance(top_logprobs_buf, torch.Tensor) else top_logprobs_buf.t
+        if not (t.get_device() == here and t.dtype is _F32 and t.numel() >= each and t.is_contiguous()):
+            _at(name, t, each, "top log-probabilities", (_F32,), here)
+        tv = t.data_ptr()
+    if top_tokens is not None:
+        if not (top_tokens.get_device() == here and top_tokens.dtype is _I32 and top_tokens.numel() >= each and top_tokens.is_contiguous()):
+            _at(name, top_tokens, each, "top tokens", (_I32,), here)
+        ti = top_tokens.data_ptr()
+    check(lib().small_b200_logprobs(num_rows, num_classes, _TYPES[x.dtype], x.data_ptr(), apart, wide, given, lp, h, top, tv, ti,
+                                    _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)))
 
 
 # --------------------------------------------------------------------------- detection head
