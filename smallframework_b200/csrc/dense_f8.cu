@@ -24,6 +24,7 @@ struct DenseArgs
 {
     int rows, K, blocks; // blocks of 128 in the reduction
     int k_tiles, r_tiles, split;
+    int first, count; // tiles of 256 x 256 that a launch of the kernel for many rows does
     int accumulate;
     float neg_scale;
     long long out_stride;
@@ -390,9 +391,12 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-// A pair of CTAs (cta_group::2) owns 256 rows by 256 outputs: each brings its 128 rows and half of the weights, 32 KB a block where a CTA by itself
+// A pair of CTAs (cta_group::2) owns 256 rows by N = 256 outputs: each brings its 128 rows and half of the weights, 32 KB a block where a CTA by itself
 // would bring 48 KB for the same products; traffic between L2 and the SMs is what bounded that (10.4 TB/s over the device).
-constexpr int MANY_N = 256, MANY_STAGE = 2 * A_BYTES, MANY_STAGES = 6, MANY_EPI = 8, MANY_THREADS = 384;
+//
+// Tiles that leave half of the pairs idle are cut to N = 128.  That brings 24 KB for half of the products, but tensor memory then holds four blocks'
+// sums, and the way from an MMA to the warps that fold and back, 900 cycles, is hidden behind three others: 0.4 of a whole tile's time.
+constexpr int MANY_STAGE = 2 * A_BYTES, MANY_STAGES = 6, MANY_EPI = 8, MANY_THREADS = 384;
 static_assert(MANY_STAGES % 2 == 0, "a buffer's blocks keep to every other stage");
 constexpr int STAGE_OUT = 32 * 128; // a warp's way out
 constexpr int MANY_SMEM = 1024 + MANY_STAGES * MANY_STAGE + MANY_EPI * STAGE_OUT;
@@ -404,12 +408,16 @@ struct TileAt
 {
     int r0, k0;
 };
+// Tile t of 256 x 256, or the half t & 1 of tile t / 2 (which may begin behind the last output).
+template <int N>
 __device__ __forceinline__ TileAt tile_at(const DenseArgs &a, int t)
 {
+    const int half = N == 128 ? t & 1 : 0;
+    t = a.first + (N == 128 ? t >> 1 : t);
     const int per_group = GROUP * a.k_tiles, g = t / per_group, in = t - g * per_group;
     const int size = min(GROUP, a.r_tiles - g * GROUP);
     const int kt = in / size;
-    return {(g * GROUP + in - kt * size) * 256, kt * MANY_N};
+    return {(g * GROUP + in - kt * size) * 256, kt * 256 + half * 128};
 }
 
 __device__ __forceinline__ void fold32(unsigned long long *acc, const uint32_t *r, unsigned long long s2)
@@ -419,21 +427,23 @@ __device__ __forceinline__ void fold32(unsigned long long *acc, const uint32_t *
         fold2(acc[c], r[2 * c], r[2 * c + 1], s2);
 }
 
-template <int TYPE>
+template <int TYPE, int N>
 __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                           const DenseArgs a, int *status)
 {
+    constexpr int BUFS = 512 / N, COLS = N / 2, BYTES = A_BYTES + N / 2 * KB; // of sums; a folding thread's outputs; of a block and CTA
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[MANY_STAGES], empty[MANY_STAGES], sum_full[2], sum_empty[2], drained[2];
+    __shared__ uint64_t full[MANY_STAGES], empty[MANY_STAGES], sum_full[BUFS], sum_empty[BUFS], drained[2];
     __shared__ uint32_t tmem_s;
     uint8_t *ring = align1024(raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = (int)cluster_ctarank(), pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
-    const int tiles = a.k_tiles * a.r_tiles;
+    const int tiles = a.count * (256 / N);
     if (tid == 0)
     {
         for (int s = 0; s < MANY_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], 2 * MANY_EPI); mbar_init(&drained[s], 1); }
+        for (int s = 0; s < BUFS; ++s) { mbar_init(&sum_full[s], 1); mbar_init(&sum_empty[s], 2 * MANY_EPI); }
+        for (int s = 0; s < 2; ++s) mbar_init(&drained[s], 1);
         fence_barrier_init();
     }
     if (warp == 3)
@@ -448,35 +458,36 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
     if (warp >= 4)
     {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_FOLD));
-        // ---- thread = one row of activations and 128 outputs, a block of weights
+        // ---- thread = one row of activations and COLS outputs of one block of weights
         const int half = (warp - 4) >> 2, lane_row = (warp & 3) * 32 + lane;
-        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * 128);
+        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * COLS);
         const uint32_t give_back = map_to_cta(sum_empty, 0);
         bool ok = true;
         unsigned i = 0;
         for (int t = pair; t < tiles && ok; t += pairs)
         {
-            const TileAt at = tile_at(a, t);
-            const int row = at.r0 + rank * 128 + lane_row, k0 = at.k0 + half * 128;
+            const TileAt at = tile_at<N>(a, t);
+            if (at.k0 >= a.K)
+                continue;
+            const int row = at.r0 + rank * 128 + lane_row, k0 = at.k0 + half * COLS;
             const float *sx = a.in_scales + (size_t)min(row, a.rows - 1) * a.blocks;
             const float *sw = a.filt_scales + (size_t)min(k0 / 128, (a.K - 1) / 128) * a.blocks;
-            unsigned long long acc[64];
+            unsigned long long acc[COLS / 2];
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
+            for (int c = 0; c < COLS / 2; ++c)
                 acc[c] = 0ull;
             // Software pipeline over the blocks: while 32 columns are folded the next 32 are on their way, across blocks too, and the next block's
             // barrier is asked one step before its answer is needed.
             float next_x = __ldg(sx), next_w = __ldg(sw); // multiplied when they are needed: until then nothing waits for them
-            uint32_t r0[32], r1[32];
-            ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[i & 1], (i >> 1) & 1, status, 111));
+            uint32_t r[2][32];
+            ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[i % BUFS], (i / BUFS) & 1, status, 111));
             if (!ok)
                 break;
             tc_fence_after_sync();
-            tmem_ld32(from + (uint32_t)((i & 1) * MANY_N), r0);
+            tmem_ld32(from + (i % BUFS) * N, r[0]);
             for (int b = 0; b < a.blocks; ++b, ++i)
             {
-                const int buf = i & 1;
-                const uint32_t src = from + (uint32_t)(buf * MANY_N);
+                const unsigned buf = i % BUFS, then = (i + 1) % BUFS, then_phase = ((i + 1) / BUFS) & 1;
                 const float s = next_x * next_w;
                 const unsigned long long s2 = (unsigned long long)__float_as_uint(s) << 32 | __float_as_uint(s);
                 const bool more = b + 1 < a.blocks;
@@ -485,33 +496,37 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                     next_x = __ldg(sx + b + 1);
                     next_w = __ldg(sw + b + 1);
                 }
-                tmem_ld_wait();
-                tmem_ld32(src + 32, r1);
-                fold32(acc, r0, s2);
-                tmem_ld_wait();
-                tmem_ld32(src + 64, r0);
-                fold32(acc + 16, r1, s2);
-                tmem_ld_wait();
-                tmem_ld32(src + 96, r1);
-                const bool ready = more && mbar_test(&sum_full[buf ^ 1], ((i + 1) >> 1) & 1);
-                fold32(acc + 32, r0, s2);
-                tmem_ld_wait();
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive_remote_relaxed(give_back + buf * 8);
-                if (more)
+                bool ready = false;
+#pragma unroll
+                for (int c = 0; c < COLS / 32; ++c)
                 {
-                    if (!__all_sync(0xffffffffu, ready))
+                    tmem_ld_wait();
+                    if (c + 1 < COLS / 32)
+                        tmem_ld32(from + buf * N + 32 * (c + 1), r[(c + 1) & 1]);
+                    else
                     {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[buf ^ 1], ((i + 1) >> 1) & 1, status, 111));
-                        if (!ok)
-                            break;
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0)
+                            mbar_arrive_remote_relaxed(give_back + buf * 8);
+                        if (more)
+                        {
+                            if (!__all_sync(0xffffffffu, ready))
+                            {
+                                ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[then], then_phase, status, 111));
+                                if (!ok)
+                                    break;
+                            }
+                            tc_fence_after_sync();
+                            tmem_ld32(from + then * N, r[0]);
+                        }
                     }
-                    tc_fence_after_sync();
-                    tmem_ld32(from + (uint32_t)((buf ^ 1) * MANY_N), r0);
+                    if (c == COLS / 32 - 2)
+                        ready = more && mbar_test(&sum_full[then], then_phase);
+                    fold32(acc + 16 * c, r[c & 1], s2);
                 }
-                fold32(acc + 48, r1, s2);
+                if (!ok)
+                    break;
             }
             if (!ok)
                 break;
@@ -520,7 +535,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, WIDE = 8 * VE;
             uint8_t *stage = ring + MANY_STAGES * MANY_STAGE + (warp - 4) * STAGE_OUT;
 #pragma unroll
-            for (int c0 = 0; c0 < 128; c0 += WIDE)
+            for (int c0 = 0; c0 < COLS; c0 += WIDE)
             {
                 if (k0 + c0 >= a.K)
                     break;
@@ -557,30 +572,36 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                     *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = w; // no two lanes of eight share banks
                 }
                 __syncwarp();
-                const int j = lane & 7, k = k0 + c0 + j * VE;
-#pragma unroll
-                for (int n = 0; n < 8; ++n)
+                const int first = at.r0 + rank * 128 + (warp & 3) * 32;
+                char *out = static_cast<char *>(a.out);
+                if (a.wide && k0 + c0 + WIDE <= a.K)
                 {
-                    const int r = n * 4 + (lane >> 3), to = at.r0 + rank * 128 + (warp & 3) * 32 + r;
-                    const uint4 w = *reinterpret_cast<const uint4 *>(stage + r * 128 + ((j ^ (r & 7)) << 4));
-                    if (to >= a.rows || k >= a.K)
-                        continue;
-                    char *dst = static_cast<char *>(a.out) + ((long long)to * a.out_stride + k) * SIZE;
-                    if (a.wide && k + VE <= a.K)
-                        *reinterpret_cast<uint4 *>(dst) = w;
-                    else
-                    {
-                        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                    const int j = lane & 7;
 #pragma unroll
-                        for (int c = 0; c < VE; ++c)
-                            if (k + c < a.K)
-                            {
-                                if (SIZE == 4)
-                                    reinterpret_cast<uint32_t *>(dst)[c] = word[c / (VE / 4)];
-                                else
-                                    reinterpret_cast<uint16_t *>(dst)[c] = (uint16_t)(word[c / (VE / 4)] >> (16 * (c & 1)));
-                            }
+                    for (int n = 0; n < 8; ++n)
+                    {
+                        const int q = n * 4 + (lane >> 3);
+                        if (first + q < a.rows)
+                            *reinterpret_cast<uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + j * VE) * SIZE) =
+                                *reinterpret_cast<const uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4));
                     }
+                }
+                else // element by element, a row at a time
+                {
+                    const int rows = min(32, a.rows - first);
+#pragma unroll 1
+                    for (int q = 0; q < rows; ++q)
+#pragma unroll
+                        for (int c = lane; c < WIDE; c += 32)
+                            if (k0 + c0 + c < a.K)
+                            {
+                                const uint8_t *src = stage + q * 128 + ((c / VE ^ (q & 7)) << 4) + c % VE * SIZE;
+                                char *dst = out + ((long long)(first + q) * a.out_stride + k0 + c0 + c) * SIZE;
+                                if (SIZE == 4)
+                                    *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
+                                else
+                                    *reinterpret_cast<uint16_t *>(dst) = *reinterpret_cast<const uint16_t *>(src);
+                            }
                 }
                 __syncwarp();
             }
@@ -597,8 +618,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             const uint32_t bars = map_to_cta(full, 0);
             for (int t = pair; t < tiles && ok; t += pairs)
             {
-                const TileAt at = tile_at(a, t);
-                const int rx = at.r0 + rank * 128, rw = at.k0 + rank * 128;
+                const TileAt at = tile_at<N>(a, t);
+                if (at.k0 >= a.K)
+                    continue;
+                const int rx = at.r0 + rank * 128, rw = at.k0 + rank * (N / 2);
                 for (int b = 0; b < a.blocks; ++b, ++i)
                 {
                     if (turn > 0)
@@ -608,7 +631,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                     if (elect_one())
                     {
                         if (rank == 0)
-                            mbar_expect_tx(&full[s], 2 * MANY_STAGE);
+                            mbar_expect_tx(&full[s], 2 * BYTES);
                         uint8_t *dst = ring + s * MANY_STAGE;
                         tma_load_2d_pair(dst, &map_x, b * KB, rx, bars + s * 8);
                         tma_load_2d_pair(dst + A_BYTES, &map_w, b * KB, rw, bars + s * 8);
@@ -631,15 +654,17 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
         }
         else if ((warp == 1 || warp == 2) && rank == 0)
         {
-            // One warp for each buffer of sums, every other block its own: what a warp does around its MMAs (500 cycles a block, most of it waiting for
-            // answers) then passes behind the other's.  The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
-            const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 256, MANY_N);
+            // Two warps, every other block its own: what a warp does around its MMAs (500 cycles a block, most of it waiting for answers) then passes
+            // behind the other's.  The whole warp walks the loop, so that descriptors stay in uniform registers; one lane issues.
+            const uint32_t idesc = make_idesc(1 /*f32*/, 0, 0, 0, 0, 256, N);
             const uint64_t first_a = make_smem_desc(smem_u32(ring), 16, 1024, 2), first_b = make_smem_desc(smem_u32(ring) + A_BYTES, 16, 1024, 2);
-            const unsigned buf = warp - 1, total = (unsigned)((tiles - pair + pairs - 1) / pairs) * (unsigned)a.blocks;
-            const uint32_t d = tmem + buf * MANY_N;
-            unsigned s = buf, turn = 0, use = 1; // stage, parity of its phase, parity of the phase before the buffer's next use
+            unsigned total = 0;
+            for (int t = pair; t < tiles; t += pairs)
+                total += tile_at<N>(a, t).k0 < a.K ? (unsigned)a.blocks : 0u;
+            const unsigned mine = warp - 1;
+            unsigned s = mine, turn = 0, buf = mine, use = 1; // stage, parity of its phase; buffer, parity of the phase before its next use
             bool ok = true;
-            for (unsigned i = buf; i < total; i += 2)
+            for (unsigned i = mine; i < total; i += 2)
             {
                 for (uint32_t n = 0; !mbar_test_both(&full[s], turn, &sum_empty[buf], use); ++n)
                     if (n >= 256) // long enough for every turn but the first ones: now the wait that gives up
@@ -653,6 +678,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                 if (elect_one())
                 {
                     const uint64_t da = first_a + s * (MANY_STAGE / 16), db = first_b + s * (MANY_STAGE / 16);
+                    const uint32_t d = tmem + buf * N;
                     tc_mma_f8_pair(d, da, db, idesc, 0u);
                     tc_mma_f8_pair(d, da + 2, db + 2, idesc, 1u);
                     tc_mma_f8_pair(d, da + 4, db + 4, idesc, 1u);
@@ -661,7 +687,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                     tc_commit_pair(&empty[s]);
                 }
                 __syncwarp();
-                use ^= 1;
+                buf += 2;
+                if (buf >= BUFS)
+                {
+                    buf -= BUFS;
+                    use ^= 1;
+                }
                 s += 2;
                 if (s >= MANY_STAGES)
                 {
@@ -672,9 +703,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             if (!__all_sync(0xffffffffu, ok))
             {
                 if (elect_one())
-                    tc_commit_pair(&drained[buf]);
+                    tc_commit_pair(&drained[mine]);
                 __syncwarp();
-                mbar_wait(&drained[buf], 0, status, 116);
+                mbar_wait(&drained[mine], 0, status, 116);
             }
         }
     }
@@ -720,6 +751,36 @@ int launch_few(DenseArgs a, const CUtensorMap &map_w, const CUtensorMap &map_x, 
     return launched("dense_f8_few_kernel");
 }
 
+template <int TYPE, int N>
+int launch_many(const DenseArgs &a, const CUtensorMap &map_x, const CUtensorMap &map_w, int *status, cudaStream_t st)
+{
+    auto kern = dense_f8_many_kernel<TYPE, N>;
+    static PerDeviceOnce configured;
+    int dev;
+    if (configured.needed(&dev))
+    {
+        SB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MANY_SMEM));
+        cudaFuncAttributes fa;
+        SB_CUDA(cudaFuncGetAttributes(&fa, kern));
+        if (fa.numRegs * MANY_THREADS < 128 * REGS_FEED + 256 * REGS_FOLD) // the split would wait for registers that the launch does not have
+            return fail(SMALL_B200_CUDA_ERROR, "dense_f8_many_kernel was built with too few registers");
+        configured.mark(dev);
+    }
+    const int pairs = std::min(a.count * (256 / N), num_sms() / 2);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * pairs));
+    cfg.blockDim = dim3(MANY_THREADS);
+    cfg.dynamicSmemBytes = MANY_SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SB_CUDA(cudaLaunchKernelEx(&cfg, kern, map_x, map_w, a, status));
+    return launched(N == 256 ? "dense_f8_many_kernel<256>" : "dense_f8_many_kernel<128>");
+}
+
 template <int TYPE>
 int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long in_stride, const void *filt, long long filt_stride, cudaStream_t st)
 {
@@ -728,12 +789,17 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
         return fail(SMALL_B200_CUDA_ERROR, "device status word not available");
     CUtensorMap map_w, map_x;
     // Microseconds that either kernel takes, fitted to 91 sizes (1 to 2048 rows, 512 to 8192 outputs and inputs): a tile and block of 128 outputs by 64 rows
-    // costs the device 2.6 ns in the one, a block of a wave of 256 x 256 tiles 0.48 us in the other.
-    // 256 rows, 4096 -> 4096: 16.4 and 20.0 us; 512 rows: 25.4 and 20.7; 256 rows, 8192 -> 1024: 12.1 and 32.9; 1024 rows: 24.9 and 33.3.
+    // costs the device 3.1 ns in the one, a block of a wave of 256 x 256 tiles 0.48 us in the other, of halves of such tiles 0.27.
+    // 256 rows, 8192 -> 1024: 12.1 and 23.0 us; 256 rows, 4096 -> 4096: 16.4 and 14.2; 128 rows: 11.0 and 14.0; 1024 rows, 8192 -> 1024: 24.9 and 23.7.
     const double units = (double)((D->K + 127LL) / 128) * ((D->rows + 63LL) / 64) * a.blocks;
     const long long pairs_of_tiles = ((D->K + 255LL) / 256) * ((D->rows + 255LL) / 256), at_once = std::max(1, num_sms() / 2);
-    const double many_us = (double)((pairs_of_tiles + at_once - 1) / at_once) * (0.48 * a.blocks + 1.2);
-    if (D->rows <= 64 || 0.0026 * units < many_us)
+    // Tiles for which there are twice as many pairs of CTAs are done in halves, a launch of its own behind whole waves (2.5 us).
+    const long long whole = pairs_of_tiles / at_once * at_once, rest = pairs_of_tiles - whole;
+    const bool halves = rest > 0 && 2 * rest <= at_once;
+    const double few_us = 4.5 + 0.0031 * units;
+    const double many_us = 4.5 + (double)(whole / at_once) * (0.48 * a.blocks + 1.5) +
+                           (rest == 0 ? 0. : halves ? 0.27 * a.blocks + 1. + (whole > 0 ? 2.5 : 0.) : 0.48 * a.blocks + 1.5);
+    if (D->rows <= 64 || few_us < many_us)
     {
         const int bn = D->rows <= 16 ? 16 : D->rows <= 32 ? 32 : 64;
         a.k_tiles = (D->K + 127) / 128;
@@ -754,38 +820,27 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
         default: return launch_few<64, TYPE>(a, map_w, map_x, status, st);
         }
     }
-    a.k_tiles = (D->K + MANY_N - 1) / MANY_N;
+    a.k_tiles = (D->K + 255) / 256;
     a.r_tiles = (D->rows + 255) / 256;
     a.split = 1;
-    if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, 128))
-        return rc;
     if (int rc = map_rows(&map_x, in, D->rows, D->C, in_stride, 128))
         return rc;
-    auto kern = dense_f8_many_kernel<TYPE>;
-    static PerDeviceOnce configured;
-    int dev;
-    if (configured.needed(&dev))
+    if (whole > 0 || !halves)
     {
-        SB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MANY_SMEM));
-        cudaFuncAttributes fa;
-        SB_CUDA(cudaFuncGetAttributes(&fa, kern));
-        if (fa.numRegs * MANY_THREADS < 128 * REGS_FEED + 256 * REGS_FOLD) // the split would wait for registers that the launch does not have
-            return fail(SMALL_B200_CUDA_ERROR, "dense_f8_many_kernel was built with too few registers");
-        configured.mark(dev);
+        if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, 128))
+            return rc;
+        a.first = 0;
+        a.count = (int)(halves ? whole : pairs_of_tiles);
+        if (int rc = launch_many<TYPE, 256>(a, map_x, map_w, status, st))
+            return rc;
     }
-    const int pairs = std::min(a.k_tiles * a.r_tiles, num_sms() / 2);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * pairs));
-    cfg.blockDim = dim3(MANY_THREADS);
-    cfg.dynamicSmemBytes = MANY_SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SB_CUDA(cudaLaunchKernelEx(&cfg, kern, map_x, map_w, a, status));
-    return launched("dense_f8_many_kernel");
+    if (!halves)
+        return SMALL_B200_OK;
+    if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, 64))
+        return rc;
+    a.first = (int)whole;
+    a.count = (int)rest;
+    return launch_many<TYPE, 128>(a, map_x, map_w, status, st);
 }
 } // namespace
 

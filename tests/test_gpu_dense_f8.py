@@ -56,10 +56,60 @@ def test_many_tiles(rows):
     run(rows, 148 * 256 + 40, 1280, "bf16", seed=3)
 
 
+# Sizes that take the kernel for many rows: whole tiles, halves of tiles (the last of which begins behind the last output), and one after the other.
+MANY = [(1100, 2500, 272, "<256>"), (300, 4100, 1040, "<128>"), (2300, 2310, 400, "<128>")]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("act,partial,bias,apart", [(0, False, False, 0), (1, False, True, 0), (2, True, True, 4), (0, True, False, 3)])
+@pytest.mark.parametrize("rows,K,C_,name", MANY)
+def test_many_rows(kind, act, partial, bias, apart, rows, K, C_, name):
+    run(rows, K, C_, kind, seed=7, bias=bias, act=act, partial=partial, stride=K + apart if apart else None)
+    assert _lib.last_kernel() == "dense_f8_many_kernel" + name
+
+
+def test_many_rows_two_at_once_and_replayed():
+    for rows, K, C_, _ in MANY:
+        x, w, other = U.operand(rows, C_, 1, 51), U.operand(K, C_, 128, 52), U.operand(rows, C_, 1, 53)
+        ys = [torch.zeros(rows, K, device="cuda", dtype=torch.bfloat16) for _ in range(4)]
+        S.Dense(K, C_, x, w, U.buffer(ys[0]), batch=rows)
+        S.Dense(K, C_, other, w, U.buffer(ys[1]), batch=rows)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        for _ in range(10):
+            for s, v, y in zip(streams, (x, other), ys[2:]):
+                S.Dense(K, C_, v, w, U.buffer(y), batch=rows, stream=s)
+        torch.cuda.synchronize()
+        assert torch.equal(ys[2], ys[0]) and torch.equal(ys[3], ys[1])
+        graph, buf = torch.cuda.CUDAGraph(), U.buffer(ys[2])
+        with torch.cuda.graph(graph):
+            S.Dense(K, C_, x, w, buf, batch=rows)
+        x.t.copy_(other.t); x.scales.copy_(other.scales)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(ys[2], ys[1]) and _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("rows,K,C_,name", MANY)
+def test_many_rows_of_nan_and_infinite_scales(rows, K, C_, name):
+    x, w = U.operand(rows, C_, 1, 31), U.operand(K, C_, 128, 32)
+    x.t.view(rows, C_).view(torch.uint8)[1, C_ - 1] = 0x7f
+    x.scales.view(rows, -1)[2, 0] = torch.inf
+    w.t.view(K, C_).view(torch.uint8)[131, 3] = 0xff
+    y = torch.empty(rows, K, device="cuda")
+    S.Dense(K, C_, x, w, U.buffer(y), batch=rows)
+    assert _lib.last_kernel() == "dense_f8_many_kernel" + name
+    want, size = U.dense(x, w)
+    assert y[1].isnan().all() and y[:, 131].isnan().all()
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf())
+    fine = want.isfinite()
+    assert ((y.double() - want).abs() <= U.dense_tolerance(want, size, C_, torch.float32))[fine].all()
+
+
 def test_fp32_sums_are_as_near_as_fp32_sums_are():
     """Over many outputs the error is far below the bound that each of them has: no bits were lost between the tensor cores and the output.
     A sum of 128 terms with one truncation each is off by at most 128 * 2^-23 of the magnitudes, the mean over outputs by far less."""
-    for rows in (8, 256):
+    for rows in (8, 256, 2048):
         off, size = run(rows, 2048, 4096, "f32", seed=21, bias=False)
         assert (off.square().sum() / size.square().sum()).sqrt() < 2.0 ** -22
 
