@@ -26,7 +26,8 @@ struct DenseArgs
     int k_tiles, r_tiles, split;
     int first, count; // tiles of 256 x 256 that a launch of the kernel for many rows does
     int accumulate;
-    float neg_scale;
+    int act;
+    float slope;
     long long out_stride;
     const float *in_scales, *filt_scales, *bias;
     void *out;
@@ -34,8 +35,13 @@ struct DenseArgs
     int wide; // rows of the output begin on 16-byte boundaries
 };
 
-// ReLU and LeakyReLU of the finished sum; unlike the convolutions' branch-free form exact for infinities too.
-__device__ __forceinline__ float activate(float v, float neg_scale) { return v > 0.f || neg_scale == 1.f ? v : (neg_scale == 0.f ? (v != v ? v : 0.f) : v * neg_scale); }
+// ReLU and LeakyReLU of the finished sum.  Infinities get what the formula gives, unlike in the convolutions' branch-free form, and NaN stays NaN.
+__device__ __forceinline__ float activate(float v, int act, float slope)
+{
+    if (act == SMALL_B200_ACT_NONE || v > 0.f)
+        return v;
+    return act == SMALL_B200_ACT_LEAKY ? v * slope : v != v ? v : 0.f;
+}
 
 template <int TYPE>
 __device__ __forceinline__ void store1(void *p, long long at, float v)
@@ -89,7 +95,7 @@ __device__ __forceinline__ void finish4(const DenseArgs &a, int row, int k, floa
                     v[c] += load1<TYPE>(a.out, at + c);
                 if (a.bias)
                     v[c] += __ldg(a.bias + k + c);
-                v[c] = activate(v[c], a.neg_scale);
+                v[c] = activate(v[c], a.act, a.slope);
             }
     }
     if (a.wide && k + 4 <= a.K)
@@ -141,6 +147,8 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
         }
         __syncwarp();
         asm volatile("bar.arrive 1, %0;" ::"n"(FEW_THREADS) : "memory");
+        previous_kernel_done();
+        next_kernel_may_start();
         if (elect_one())
             for (int i = 0; i < G::STAGES && i < n; ++i)
                 load(i, i);
@@ -184,7 +192,13 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
     if (warp != 4)
         asm volatile("bar.sync 1, %0;" ::"n"(FEW_THREADS) : "memory");
     __syncwarp();
-    cluster_arrive_relaxed(); // this CTA's inbox can be written to: its barrier has been made and fenced
+    if (a.split > 1)
+        cluster_arrive_relaxed(); // this CTA's inbox can be written to: its barrier has been made and fenced
+    if (warp != 4)
+    {
+        previous_kernel_done();
+        next_kernel_may_start();
+    }
     tc_fence_after_sync();
     const uint32_t tmem = tmem_s;
     unsigned long long acc[BN / 2]; // of the folding warps
@@ -340,31 +354,45 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
     __syncwarp();
     // ---- every CTA of the cluster has a share of the rows: the others send it what they have of them (a wait that gave up leaves rubbish, which
     // the status word tells)
-    cluster_wait(); // all inboxes can be written to
     const int per = BN / a.split;
-    if (warp < 4)
+    bool all = true;
+    if (a.split == 1)
     {
-        const unsigned long long *mine = inbox + rank * (per / 2) * 128 + tid;
-        int to = 0, left = per; // of the share that is being sent
-        uint32_t at = map_to_cta(mine, 0), bar = map_to_cta(&delivered, 0);
-#pragma unroll
-        for (int c = 0; c < BN; c += 2)
+        if (warp < 4)
         {
-            st_async_b64(at, acc[c / 2], bar);
-            at += 128 * 8;
-            left -= 2;
-            if (left == 0 && c + 2 < BN)
+#pragma unroll
+            for (int c = 0; c < BN; c += 2)
+                inbox[c / 2 * 128 + tid] = acc[c / 2];
+        }
+        __syncthreads();
+    }
+    else
+    {
+        cluster_wait(); // all inboxes can be written to
+        if (warp < 4)
+        {
+            const unsigned long long *mine = inbox + rank * (per / 2) * 128 + tid;
+            int to = 0, left = per; // of the share that is being sent
+            uint32_t at = map_to_cta(mine, 0), bar = map_to_cta(&delivered, 0);
+#pragma unroll
+            for (int c = 0; c < BN; c += 2)
             {
-                left = per;
-                ++to;
-                at = map_to_cta(mine, to);
-                bar = map_to_cta(&delivered, to);
+                st_async_b64(at, acc[c / 2], bar);
+                at += 128 * 8;
+                left -= 2;
+                if (left == 0 && c + 2 < BN)
+                {
+                    left = per;
+                    ++to;
+                    at = map_to_cta(mine, to);
+                    bar = map_to_cta(&delivered, to);
+                }
             }
         }
+        __syncwarp();
+        cluster_arrive_relaxed(); // nothing more is sent
+        all = mbar_wait_cluster(&delivered, 0, status, 109);
     }
-    __syncwarp();
-    cluster_arrive_relaxed(); // nothing more is sent
-    const bool all = mbar_wait_cluster(&delivered, 0, status, 109);
     // the parts in the order of the reduction, then bias, activation and the one rounding: a warp takes two rows, a lane four outputs
     const int k = kt * 128 + 4 * lane;
     for (int p = warp; 2 * p < per; p += FEW_THREADS / 32)
@@ -383,11 +411,14 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
         if (k < a.K && row + 1 < a.rows)
             finish4<TYPE>(a, row + 1, k, v);
     }
-    __syncwarp();
-    cluster_wait(); // this CTA's shared memory stays while anybody may send to it
-    if (!all)
-        for (int i = 0; i < 1000; ++i)
-            __nanosleep(1000); // and what was sent last is on its way for less than that
+    if (a.split > 1)
+    {
+        __syncwarp();
+        cluster_wait(); // this CTA's shared memory stays while anybody may send to it
+        if (!all)
+            for (int i = 0; i < 1000; ++i)
+                __nanosleep(1000); // and what was sent last is on its way for less than that
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -453,6 +484,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
     cluster_arrive_relaxed(); // the barriers have been made and fenced
     cluster_wait();
     tc_fence_after_sync();
+    previous_kernel_done();
+    next_kernel_may_start();
     const uint32_t tmem = tmem_s;
 
     if (warp >= 4)
@@ -560,7 +593,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                                 v[c] += load1<TYPE>(a.out, (long long)row * a.out_stride + k);
                             if (a.bias && k < a.K)
                                 v[c] += __ldg(a.bias + k);
-                            v[c] = activate(v[c], a.neg_scale);
+                            v[c] = activate(v[c], a.act, a.slope);
                         }
                     }
                     uint4 w;
@@ -737,17 +770,8 @@ int launch_few(DenseArgs a, const CUtensorMap &map_w, const CUtensorMap &map_x, 
         SB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
         configured.mark(dev);
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.k_tiles * a.r_tiles * a.split));
-    cfg.blockDim = dim3(FEW_THREADS);
-    cfg.dynamicSmemBytes = G::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SB_CUDA(cudaLaunchKernelEx(&cfg, kern, map_w, map_x, a, status));
+    const Launch l((unsigned)(a.k_tiles * a.r_tiles * a.split), FEW_THREADS, G::SMEM, st, a.split > 1 ? (unsigned)a.split : 0u);
+    SB_CUDA(cudaLaunchKernelEx(&l.cfg, kern, map_w, map_x, a, status));
     return launched("dense_f8_few_kernel");
 }
 
@@ -767,17 +791,8 @@ int launch_many(const DenseArgs &a, const CUtensorMap &map_x, const CUtensorMap 
         configured.mark(dev);
     }
     const int pairs = std::min(a.count * (256 / N), num_sms() / 2);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * pairs));
-    cfg.blockDim = dim3(MANY_THREADS);
-    cfg.dynamicSmemBytes = MANY_SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SB_CUDA(cudaLaunchKernelEx(&cfg, kern, map_x, map_w, a, status));
+    const Launch l((unsigned)(2 * pairs), MANY_THREADS, MANY_SMEM, st, 2);
+    SB_CUDA(cudaLaunchKernelEx(&l.cfg, kern, map_x, map_w, a, status));
     return launched(N == 256 ? "dense_f8_many_kernel<256>" : "dense_f8_many_kernel<128>");
 }
 
@@ -875,7 +890,7 @@ extern "C" int small_b200_dense_f8(const small_b200_dense *D, const void *in, co
         return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: too many tiles.");
     DenseArgs a = {};
     a.rows = D->rows; a.K = D->K; a.blocks = (D->C + KB - 1) / KB;
-    a.accumulate = D->accumulate; a.neg_scale = D->act == SMALL_B200_ACT_RELU ? 0.f : D->act == SMALL_B200_ACT_LEAKY ? D->slope : 1.f;
+    a.accumulate = D->accumulate; a.act = D->act; a.slope = D->slope;
     a.out_stride = out_stride; a.in_scales = in_scales; a.filt_scales = filt_scales; a.bias = bias; a.out = out;
     a.finish = bias || D->accumulate || D->act != SMALL_B200_ACT_NONE;
     a.wide = !off(out, 16) && out_stride * size % 16 == 0;

@@ -269,6 +269,8 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
         __syncwarp();
         cluster_arrive_relaxed();
     }
+    previous_kernel_done();
+    next_kernel_may_start();
     // the given class's logit, asked for before everything else
     long long token = -1;
     float given = 0.f;
@@ -672,16 +674,8 @@ int launch_logprobs(const LogpArgs &a, const void *logits, const void *tokens, f
     int *status = device_status_ptr();
     if (!status)
         return fail(SMALL_B200_CUDA_ERROR, "device status word not available");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(WARPS == 1 ? (a.rows + 7) / 8 : a.rows * a.split));
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    SB_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<TYPE, WARPS>, a, logits, tokens, logprobs, entropy, top_logprobs, (int *)top_tokens, status));
+    const Launch l((unsigned)(WARPS == 1 ? (a.rows + 7) / 8 : a.rows * a.split), 256, 0, st, a.split > 1 ? (unsigned)a.split : 0u);
+    SB_CUDA(cudaLaunchKernelEx(&l.cfg, logprobs_kernel<TYPE, WARPS>, a, logits, tokens, logprobs, entropy, top_logprobs, (int *)top_tokens, status));
     return launched("logprobs_kernel");
 }
 } // namespace

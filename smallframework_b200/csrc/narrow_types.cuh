@@ -14,7 +14,32 @@ inline int type_size(int type)
     return type == SMALL_B200_TYPE_F32 ? 4 : (type == SMALL_B200_TYPE_BF16 || type == SMALL_B200_TYPE_F16) ? 2 : 0;
 }
 
+// A launch that may come up while the kernel before it in its stream ends: clusters of `cluster` CTAs along x, 0 for none (the kernels
+// then use no cluster instructions: stores to shared::cluster and cluster barriers of a cluster of one raised illegal instructions).  Its kernel sets itself up, calls
+// previous_kernel_done() before it touches global memory, and next_kernel_may_start() once: what comes behind it waits for the whole of it all the same.
+// Twenty dependent calls in a row take 1.5 to 2 us less each (quantisation of one row of 4096: PDL_A to PDL_B us).
+struct Launch
+{
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    Launch(unsigned grid, unsigned threads, size_t smem, cudaStream_t st, unsigned cluster = 0)
+    {
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = cluster > 0 ? 2 : 1;
+    }
+};
+
 #ifdef __CUDACC__
+__device__ __forceinline__ void previous_kernel_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // The two 16-bit floats of a word.
 template <int TYPE>
 __device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi)

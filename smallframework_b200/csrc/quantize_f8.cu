@@ -240,6 +240,8 @@ __global__ void __launch_bounds__(ROW_THREADS, TYPE == SMALL_B200_TYPE_F32 ? 4 :
     const int lane = threadIdx.x & 15;
     const long long u0 = (long long)blockIdx.x * (GROUPS * UNITS) + (threadIdx.x >> 4);
     Raw8<TYPE> r[UNITS];
+    previous_kernel_done();
+    next_kernel_may_start();
     if (FLAT && ((long long)blockIdx.x + 1) * (GROUPS * UNITS) <= a.units)
     {
         const char *p = static_cast<const char *>(in) + (u0 * 128 + lane * 8) * SIZE;
@@ -279,6 +281,8 @@ __global__ void __launch_bounds__(256) quantize_square_f8_kernel(const QuantArgs
     const int br = a.by_blocks.div((int)blockIdx.x), bc = (int)blockIdx.x - br * a.blocks;
     const int c = bc * 128 + lane * 8;
     float x[8][8];
+    previous_kernel_done();
+    next_kernel_may_start();
 #pragma unroll
     for (int j = 0; j < 8; ++j)
     {
@@ -329,14 +333,15 @@ int launch_quantize(const QuantArgs &a, int block_rows, const void *in, uint8_t 
 {
     if (block_rows == 128)
     {
-        quantize_square_f8_kernel<TYPE, VEC><<<(unsigned)a.units, 256, 0, st>>>(a, in, out, scales);
+        const Launch l((unsigned)a.units, 256, 0, st);
+        SB_CUDA(cudaLaunchKernelEx(&l.cfg, quantize_square_f8_kernel<TYPE, VEC>, a, in, out, scales));
         return launched("quantize_square_f8_kernel");
     }
-    const unsigned grid = (unsigned)((a.units + GROUPS * UNITS - 1) / (GROUPS * UNITS));
+    const Launch l((unsigned)((a.units + GROUPS * UNITS - 1) / (GROUPS * UNITS)), ROW_THREADS, 0, st);
     if (VEC && a.stride == a.columns && a.columns % 128 == 0)
-        quantize_rows_f8_kernel<TYPE, VEC, VEC><<<grid, ROW_THREADS, 0, st>>>(a, in, out, scales);
+        SB_CUDA(cudaLaunchKernelEx(&l.cfg, quantize_rows_f8_kernel<TYPE, VEC, VEC>, a, in, out, scales));
     else
-        quantize_rows_f8_kernel<TYPE, VEC, false><<<grid, ROW_THREADS, 0, st>>>(a, in, out, scales);
+        SB_CUDA(cudaLaunchKernelEx(&l.cfg, quantize_rows_f8_kernel<TYPE, VEC, false>, a, in, out, scales));
     return launched("quantize_rows_f8_kernel");
 }
 } // namespace
