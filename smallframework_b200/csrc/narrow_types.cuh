@@ -22,14 +22,14 @@ struct Launch
 {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    Launch(unsigned grid, unsigned threads, size_t smem, cudaStream_t st, unsigned cluster = 0)
+    Launch(unsigned grid, unsigned threads, size_t smem, cudaStream_t st, unsigned cluster = 0, bool early = true)
     {
         cfg.gridDim = dim3(grid);
         cfg.blockDim = dim3(threads);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = st;
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
         attr[1].id = cudaLaunchAttributeClusterDimension;
         attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;

@@ -333,11 +333,11 @@ int launch_quantize(const QuantArgs &a, int block_rows, const void *in, uint8_t 
 {
     if (block_rows == 128)
     {
-        const Launch l((unsigned)a.units, 256, 0, st);
+        const Launch l((unsigned)a.units, 256, 0, st, 0, a.units <= 2 * num_sms());
         SB_CUDA(cudaLaunchKernelEx(&l.cfg, quantize_square_f8_kernel<TYPE, VEC>, a, in, out, scales));
         return launched("quantize_square_f8_kernel");
     }
-    const Launch l((unsigned)((a.units + GROUPS * UNITS - 1) / (GROUPS * UNITS)), ROW_THREADS, 0, st);
+    const Launch l((unsigned)((a.units + GROUPS * UNITS - 1) / (GROUPS * UNITS)), ROW_THREADS, 0, st, 0, a.units <= 4LL * num_sms() * GROUPS * UNITS);
     if (VEC && a.stride == a.columns && a.columns % 128 == 0)
         SB_CUDA(cudaLaunchKernelEx(&l.cfg, quantize_rows_f8_kernel<TYPE, VEC, VEC>, a, in, out, scales));
     else
