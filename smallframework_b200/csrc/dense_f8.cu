@@ -10,6 +10,7 @@
 //          the reduction cut among the CTAs of a cluster where output tiles are few; the parts are added over distributed shared memory, in order.
 //   many   128 rows of activations are the lanes, 256 outputs the columns.  The tensor cores bound it; one CTA an SM takes tile after tile.
 #include <algorithm>
+#include <type_traits>
 
 #include "narrow_types.cuh"
 #include "tc_common.cuh"
@@ -458,6 +459,27 @@ __device__ __forceinline__ void fold32(unsigned long long *acc, const uint32_t *
         fold2(acc[c], r[2 * c], r[2 * c + 1], s2);
 }
 
+template <int SIZE>
+__device__ __forceinline__ void copy_element(void *to, const void *from)
+{
+    if (SIZE == 4)
+        *static_cast<uint32_t *>(to) = *static_cast<const uint32_t *>(from);
+    else
+        *static_cast<uint16_t *>(to) = *static_cast<const uint16_t *>(from);
+}
+// WIDE columns from column k of a warp's 32 rows, element by element and a row at a time, as far as the output goes.
+template <int WIDE, int SIZE, class F>
+__device__ __forceinline__ void element_by_element(const DenseArgs &a, char *out, int first, int k, F each)
+{
+    const int lane = threadIdx.x & 31, rows = min(32, a.rows - first);
+#pragma unroll 1
+    for (int q = 0; q < rows; ++q)
+#pragma unroll
+        for (int c = lane; c < WIDE; c += 32)
+            if (k + c < a.K)
+                each(q, c, out + ((long long)(first + q) * a.out_stride + k + c) * SIZE);
+}
+
 template <int TYPE, int N>
 __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                           const DenseArgs a, int *status)
@@ -567,77 +589,114 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             // 16-byte store of a warp touches 32 lines, and a tile took 5000 cycles.
             constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, WIDE = 8 * VE;
             uint8_t *stage = ring + MANY_STAGES * MANY_STAGE + (warp - 4) * STAGE_OUT;
-#pragma unroll
-            for (int c0 = 0; c0 < COLS; c0 += WIDE)
-            {
-                if (k0 + c0 >= a.K)
-                    break;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
+            const int first = at.r0 + rank * 128 + (warp & 3) * 32; // row of the warp
+            char *out = static_cast<char *>(a.out);
+            auto send = [&](auto finish) {
+                constexpr bool FINISH = decltype(finish)::value;
+                float bias[COLS / 32]; // of columns lane, lane + 32, ..., handed round: loads of all of them by every thread were 5 us a tile
+                if (FINISH)
                 {
-                    float v[VE];
 #pragma unroll
-                    for (int c = 0; c < VE; c += 2)
-                    {
-                        const float2 f = pair_of(acc[(c0 + j * VE + c) / 2]);
-                        v[c] = f.x;
-                        v[c + 1] = f.y;
-                    }
-                    if (a.finish)
-                    {
+                    for (int c = 0; c < COLS / 32; ++c)
+                        bias[c] = a.bias && k0 + 32 * c + lane < a.K ? __ldg(a.bias + k0 + 32 * c + lane) : 0.f;
+                }
 #pragma unroll
-                        for (int c = 0; c < VE; ++c)
+                for (int c0 = 0; c0 < COLS; c0 += WIDE)
+                {
+                    if (k0 + c0 >= a.K)
+                        break;
+                    const bool wide = a.wide && k0 + c0 + WIDE <= a.K;
+                    if (FINISH && a.accumulate) // the old values come in the way the new ones go out
+                    {
+                        if (wide)
                         {
-                            const int k = k0 + c0 + j * VE + c;
-                            if (a.accumulate && k < a.K && row < a.rows)
-                                v[c] += load1<TYPE>(a.out, (long long)row * a.out_stride + k);
-                            if (a.bias && k < a.K)
-                                v[c] += __ldg(a.bias + k);
-                            v[c] = activate(v[c], a.act, a.slope);
+#pragma unroll
+                            for (int n = 0; n < 8; ++n)
+                            {
+                                const int q = n * 4 + (lane >> 3), j = lane & 7;
+                                if (first + q < a.rows)
+                                    *reinterpret_cast<uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4)) =
+                                        *reinterpret_cast<const uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + j * VE) * SIZE);
+                            }
+                        }
+                        else
+                            element_by_element<WIDE, SIZE>(a, out, first, k0 + c0, [&](int q, int c, char *there) {
+                                copy_element<SIZE>(stage + q * 128 + ((c / VE ^ (q & 7)) << 4) + c % VE * SIZE, there);
+                            });
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                    {
+                        uint4 *slot = reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)); // no two lanes of eight share banks
+                        float v[VE];
+#pragma unroll
+                        for (int c = 0; c < VE; c += 2)
+                        {
+                            const float2 f = pair_of(acc[(c0 + j * VE + c) / 2]);
+                            v[c] = f.x;
+                            v[c + 1] = f.y;
+                        }
+                        if (FINISH && a.accumulate)
+                        {
+                            float old[VE];
+                            const uint4 w = *slot;
+                            if (TYPE == SMALL_B200_TYPE_F32)
+                            {
+                                old[0] = __uint_as_float(w.x); old[1] = __uint_as_float(w.y); old[2] = __uint_as_float(w.z); old[3] = __uint_as_float(w.w);
+                            }
+                            else
+                            {
+                                unpack2<TYPE>(w.x, old[0], old[1]); unpack2<TYPE>(w.y, old[2], old[3]);
+                                unpack2<TYPE>(w.z, old[VE - 4], old[VE - 3]); unpack2<TYPE>(w.w, old[VE - 2], old[VE - 1]);
+                            }
+#pragma unroll
+                            for (int c = 0; c < VE; ++c)
+                                v[c] += old[c];
+                        }
+                        if (FINISH && a.bias)
+                        {
+#pragma unroll
+                            for (int c = 0; c < VE; ++c)
+                                v[c] += __shfl_sync(0xffffffffu, bias[(c0 + j * VE + c) / 32], (c0 + j * VE + c) % 32);
+                        }
+                        if (FINISH && a.act != SMALL_B200_ACT_NONE)
+                        {
+#pragma unroll
+                            for (int c = 0; c < VE; ++c)
+                                v[c] = activate(v[c], a.act, a.slope);
+                        }
+                        uint4 w;
+                        if (TYPE == SMALL_B200_TYPE_F32)
+                            w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                        else
+                            w = make_uint4(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]), pack2<TYPE>(v[VE - 4], v[VE - 3]),
+                                           pack2<TYPE>(v[VE - 2], v[VE - 1]));
+                        *slot = w;
+                    }
+                    __syncwarp();
+                    if (wide)
+                    {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+                        {
+                            const int q = n * 4 + (lane >> 3), j = lane & 7;
+                            if (first + q < a.rows)
+                                *reinterpret_cast<uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + j * VE) * SIZE) =
+                                    *reinterpret_cast<const uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4));
                         }
                     }
-                    uint4 w;
-                    if (TYPE == SMALL_B200_TYPE_F32)
-                        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
                     else
-                        w = make_uint4(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]), pack2<TYPE>(v[VE - 4], v[VE - 3]),
-                                       pack2<TYPE>(v[VE - 2], v[VE - 1]));
-                    *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = w; // no two lanes of eight share banks
+                        element_by_element<WIDE, SIZE>(a, out, first, k0 + c0, [&](int q, int c, char *there) {
+                            copy_element<SIZE>(there, stage + q * 128 + ((c / VE ^ (q & 7)) << 4) + c % VE * SIZE);
+                        });
+                    __syncwarp();
                 }
-                __syncwarp();
-                const int first = at.r0 + rank * 128 + (warp & 3) * 32;
-                char *out = static_cast<char *>(a.out);
-                if (a.wide && k0 + c0 + WIDE <= a.K)
-                {
-                    const int j = lane & 7;
-#pragma unroll
-                    for (int n = 0; n < 8; ++n)
-                    {
-                        const int q = n * 4 + (lane >> 3);
-                        if (first + q < a.rows)
-                            *reinterpret_cast<uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + j * VE) * SIZE) =
-                                *reinterpret_cast<const uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4));
-                    }
-                }
-                else // element by element, a row at a time
-                {
-                    const int rows = min(32, a.rows - first);
-#pragma unroll 1
-                    for (int q = 0; q < rows; ++q)
-#pragma unroll
-                        for (int c = lane; c < WIDE; c += 32)
-                            if (k0 + c0 + c < a.K)
-                            {
-                                const uint8_t *src = stage + q * 128 + ((c / VE ^ (q & 7)) << 4) + c % VE * SIZE;
-                                char *dst = out + ((long long)(first + q) * a.out_stride + k0 + c0 + c) * SIZE;
-                                if (SIZE == 4)
-                                    *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
-                                else
-                                    *reinterpret_cast<uint16_t *>(dst) = *reinterpret_cast<const uint16_t *>(src);
-                            }
-                }
-                __syncwarp();
-            }
+            };
+            if (a.finish) // (asked for every value, a bias, an activation and old values took 0.7 us a tile that has none)
+                send(std::true_type());
+            else
+                send(std::false_type());
         }
     }
     else
