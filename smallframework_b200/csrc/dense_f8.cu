@@ -10,7 +10,6 @@
 //          the reduction cut among the CTAs of a cluster where output tiles are few; the parts are added over distributed shared memory, in order.
 //   many   128 rows of activations are the lanes, 256 outputs the columns.  The tensor cores bound it; one CTA an SM takes tile after tile.
 #include <algorithm>
-#include <type_traits>
 
 #include "narrow_types.cuh"
 #include "tc_common.cuh"
@@ -36,12 +35,14 @@ struct DenseArgs
     int wide; // rows of the output begin on 16-byte boundaries
 };
 
-// ReLU and LeakyReLU of the finished sum.  Infinities get what the formula gives, unlike in the convolutions' branch-free form, and NaN stays NaN.
-__device__ __forceinline__ float activate(float v, int act, float slope)
+// ReLU and LeakyReLU of the finished sum, without branches (`below`: the slope, 1 for no activation).  Infinities get what the formula gives, unlike in the
+// convolutions' form, and NaN stays NaN.
+__device__ __forceinline__ float activate(float v, bool relu, float below)
 {
-    if (act == SMALL_B200_ACT_NONE || v > 0.f)
-        return v;
-    return act == SMALL_B200_ACT_LEAKY ? v * slope : v != v ? v : 0.f;
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+    const float l = v > 0.f ? v : v * below;
+    return relu ? r : l;
 }
 
 template <int TYPE>
@@ -80,39 +81,66 @@ struct Few
 };
 constexpr int FEW_THREADS = 7 * 32;
 
-// Four consecutive outputs of a row.
-template <int TYPE>
-__device__ __forceinline__ void finish4(const DenseArgs &a, int row, int k, float4 v4)
+__device__ __forceinline__ float4 bias4(const DenseArgs &a, int k)
 {
-    float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.bias)
+    {
+        const int last = a.K - 1;
+        b = make_float4(__ldg(a.bias + min(k, last)), __ldg(a.bias + min(k + 1, last)), __ldg(a.bias + min(k + 2, last)), __ldg(a.bias + min(k + 3, last)));
+    }
+    return b;
+}
+// Four consecutive outputs of a row as they are, and to where they are; the first `here` of them where they are not on a boundary of their own.
+template <int TYPE>
+__device__ __forceinline__ float4 load_few(const void *p, long long at, int here)
+{
+    return make_float4(load1<TYPE>(p, at), here > 1 ? load1<TYPE>(p, at + 1) : 0.f, here > 2 ? load1<TYPE>(p, at + 2) : 0.f,
+                       here > 3 ? load1<TYPE>(p, at + 3) : 0.f);
+}
+template <int TYPE>
+__device__ __forceinline__ void store_few(void *p, long long at, int here, float4 v)
+{
+    store1<TYPE>(p, at, v.x);
+    if (here > 1)
+        store1<TYPE>(p, at + 1, v.y);
+    if (here > 2)
+        store1<TYPE>(p, at + 2, v.z);
+    if (here > 3)
+        store1<TYPE>(p, at + 3, v.w);
+}
+template <int TYPE>
+__device__ __forceinline__ float4 load4(const DenseArgs &a, int row, int k)
+{
     const long long at = (long long)row * a.out_stride + k;
-    if (a.finish)
-    {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (k + c < a.K)
-            {
-                if (a.accumulate)
-                    v[c] += load1<TYPE>(a.out, at + c);
-                if (a.bias)
-                    v[c] += __ldg(a.bias + k + c);
-                v[c] = activate(v[c], a.act, a.slope);
-            }
-    }
-    if (a.wide && k + 4 <= a.K)
-    {
-        if (TYPE == SMALL_B200_TYPE_F32)
-            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-        else
-            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
-    }
+    if (!(a.wide && k + 4 <= a.K))
+        return load_few<TYPE>(a.out, at, a.K - k);
+    if (TYPE == SMALL_B200_TYPE_F32)
+        return *reinterpret_cast<const float4 *>(static_cast<const float *>(a.out) + at);
+    const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.out) + at);
+    float4 v;
+    unpack2<TYPE>(w.x, v.x, v.y);
+    unpack2<TYPE>(w.y, v.z, v.w);
+    return v;
+}
+template <int TYPE>
+__device__ __forceinline__ void store4(const DenseArgs &a, int row, int k, float4 v)
+{
+    const long long at = (long long)row * a.out_stride + k;
+    if (!(a.wide && k + 4 <= a.K))
+        store_few<TYPE>(a.out, at, a.K - k, v);
+    else if (TYPE == SMALL_B200_TYPE_F32)
+        *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = v;
     else
-    {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (k + c < a.K)
-                store1<TYPE>(a.out, at + c, v[c]);
-    }
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(pack2<TYPE>(v.x, v.y), pack2<TYPE>(v.z, v.w));
+}
+// The sum with the old value, the bias and the activation.
+__device__ __forceinline__ float4 finished(const DenseArgs &a, float4 sum, float4 old, float4 bias)
+{
+    const bool relu = a.act == SMALL_B200_ACT_RELU;
+    const float below = a.act == SMALL_B200_ACT_LEAKY ? a.slope : 1.f;
+    return make_float4(activate(sum.x + old.x + bias.x, relu, below), activate(sum.y + old.y + bias.y, relu, below),
+                       activate(sum.z + old.z + bias.z, relu, below), activate(sum.w + old.w + bias.w, relu, below));
 }
 
 template <int BN, int TYPE>
@@ -396,6 +424,7 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
     }
     // the parts in the order of the reduction, then bias, activation and the one rounding: a warp takes two rows, a lane four outputs
     const int k = kt * 128 + 4 * lane;
+    const float4 bias = bias4(a, k);
     for (int p = warp; 2 * p < per; p += FEW_THREADS / 32)
     {
         float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
@@ -407,10 +436,11 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
             u.z += y.x; v.z += y.y; u.w += y.z; v.w += y.w;
         }
         const int row = r0 + rank * per + 2 * p;
+        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
         if (k < a.K && row < a.rows)
-            finish4<TYPE>(a, row, k, u);
+            store4<TYPE>(a, row, k, finished(a, u, a.accumulate ? load4<TYPE>(a, row, k) : none, bias));
         if (k < a.K && row + 1 < a.rows)
-            finish4<TYPE>(a, row + 1, k, v);
+            store4<TYPE>(a, row + 1, k, finished(a, v, a.accumulate ? load4<TYPE>(a, row + 1, k) : none, bias));
     }
     if (a.split > 1)
     {
@@ -459,25 +489,35 @@ __device__ __forceinline__ void fold32(unsigned long long *acc, const uint32_t *
         fold2(acc[c], r[2 * c], r[2 * c + 1], s2);
 }
 
-template <int SIZE>
-__device__ __forceinline__ void copy_element(void *to, const void *from)
+// Eight of a warp's 32 rows, four columns from k on, out of its shared memory.  In line and in a loop: a call keeps what it saves, and long code what does not
+// fit, in local memory, which beside 227 KB of shared memory is hardly cached (8 us a tile).
+template <int TYPE>
+__device__ __forceinline__ void finish_rows(const DenseArgs &a, const uint8_t *stage, int first, int k, float4 bias)
 {
-    if (SIZE == 4)
-        *static_cast<uint32_t *>(to) = *static_cast<const uint32_t *>(from);
-    else
-        *static_cast<uint16_t *>(to) = *static_cast<const uint16_t *>(from);
-}
-// WIDE columns from column k of a warp's 32 rows, element by element and a row at a time, as far as the output goes.
-template <int WIDE, int SIZE, class F>
-__device__ __forceinline__ void element_by_element(const DenseArgs &a, char *out, int first, int k, F each)
-{
-    const int lane = threadIdx.x & 31, rows = min(32, a.rows - first);
+    const int lane = threadIdx.x & 31;
+    if (k >= a.K)
+        return;
+    constexpr int TOGETHER = 2; // short code: what a tile runs through once has to be fetched, 4 us a launch with four at a time
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-    for (int q = 0; q < rows; ++q)
+    for (int at = 0; at < 8; at += TOGETHER)
+    {
+        float4 old[TOGETHER];
+        int row[TOGETHER];
 #pragma unroll
-        for (int c = lane; c < WIDE; c += 32)
-            if (k + c < a.K)
-                each(q, c, out + ((long long)(first + q) * a.out_stride + k + c) * SIZE);
+        for (int n = 0; n < TOGETHER; ++n)
+        {
+            row[n] = (lane >> 3) + 4 * (at + n);
+            old[n] = a.accumulate && first + row[n] < a.rows ? load4<TYPE>(a, first + row[n], k) : none;
+        }
+#pragma unroll
+        for (int n = 0; n < TOGETHER; ++n)
+        {
+            const float4 sum = *reinterpret_cast<const float4 *>(stage + row[n] * 128 + (((lane & 7) ^ (row[n] & 7)) << 4));
+            if (first + row[n] < a.rows)
+                store4<TYPE>(a, first + row[n], k, finished(a, sum, old[n], bias));
+        }
+    }
 }
 
 template <int TYPE, int N>
@@ -591,112 +631,86 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             uint8_t *stage = ring + MANY_STAGES * MANY_STAGE + (warp - 4) * STAGE_OUT;
             const int first = at.r0 + rank * 128 + (warp & 3) * 32; // row of the warp
             char *out = static_cast<char *>(a.out);
-            auto send = [&](auto finish) {
-                constexpr bool FINISH = decltype(finish)::value;
-                float bias[COLS / 32]; // of columns lane, lane + 32, ..., handed round: loads of all of them by every thread were 5 us a tile
-                if (FINISH)
-                {
+            if (a.finish)
+            {
+                // With a bias, an activation or old values: the sums go in as they are, 32 columns at a time, and a lane finishes four columns of eight
+                // rows.  (Every thread by itself for its row's bias was 5 us a tile.)
+                float4 bias[COLS / 32];
 #pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c)
-                        bias[c] = a.bias && k0 + 32 * c + lane < a.K ? __ldg(a.bias + k0 + 32 * c + lane) : 0.f;
-                }
+                for (int c0 = 0; c0 < COLS; c0 += 32)
+                    bias[c0 / 32] = bias4(a, k0 + c0 + 4 * (lane & 7));
 #pragma unroll
-                for (int c0 = 0; c0 < COLS; c0 += WIDE)
+                for (int c0 = 0; c0 < COLS; c0 += 32)
                 {
                     if (k0 + c0 >= a.K)
                         break;
-                    const bool wide = a.wide && k0 + c0 + WIDE <= a.K;
-                    if (FINISH && a.accumulate) // the old values come in the way the new ones go out
-                    {
-                        if (wide)
-                        {
-#pragma unroll
-                            for (int n = 0; n < 8; ++n)
-                            {
-                                const int q = n * 4 + (lane >> 3), j = lane & 7;
-                                if (first + q < a.rows)
-                                    *reinterpret_cast<uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4)) =
-                                        *reinterpret_cast<const uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + j * VE) * SIZE);
-                            }
-                        }
-                        else
-                            element_by_element<WIDE, SIZE>(a, out, first, k0 + c0, [&](int q, int c, char *there) {
-                                copy_element<SIZE>(stage + q * 128 + ((c / VE ^ (q & 7)) << 4) + c % VE * SIZE, there);
-                            });
-                        __syncwarp();
-                    }
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                     {
-                        uint4 *slot = reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)); // no two lanes of eight share banks
-                        float v[VE];
-#pragma unroll
-                        for (int c = 0; c < VE; c += 2)
-                        {
-                            const float2 f = pair_of(acc[(c0 + j * VE + c) / 2]);
-                            v[c] = f.x;
-                            v[c + 1] = f.y;
-                        }
-                        if (FINISH && a.accumulate)
-                        {
-                            float old[VE];
-                            const uint4 w = *slot;
-                            if (TYPE == SMALL_B200_TYPE_F32)
-                            {
-                                old[0] = __uint_as_float(w.x); old[1] = __uint_as_float(w.y); old[2] = __uint_as_float(w.z); old[3] = __uint_as_float(w.w);
-                            }
-                            else
-                            {
-                                unpack2<TYPE>(w.x, old[0], old[1]); unpack2<TYPE>(w.y, old[2], old[3]);
-                                unpack2<TYPE>(w.z, old[VE - 4], old[VE - 3]); unpack2<TYPE>(w.w, old[VE - 2], old[VE - 1]);
-                            }
-#pragma unroll
-                            for (int c = 0; c < VE; ++c)
-                                v[c] += old[c];
-                        }
-                        if (FINISH && a.bias)
-                        {
-#pragma unroll
-                            for (int c = 0; c < VE; ++c)
-                                v[c] += __shfl_sync(0xffffffffu, bias[(c0 + j * VE + c) / 32], (c0 + j * VE + c) % 32);
-                        }
-                        if (FINISH && a.act != SMALL_B200_ACT_NONE)
-                        {
-#pragma unroll
-                            for (int c = 0; c < VE; ++c)
-                                v[c] = activate(v[c], a.act, a.slope);
-                        }
-                        uint4 w;
-                        if (TYPE == SMALL_B200_TYPE_F32)
-                            w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-                        else
-                            w = make_uint4(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]), pack2<TYPE>(v[VE - 4], v[VE - 3]),
-                                           pack2<TYPE>(v[VE - 2], v[VE - 1]));
-                        *slot = w;
+                        const float2 u = pair_of(acc[c0 / 2 + 2 * j]), v = pair_of(acc[c0 / 2 + 2 * j + 1]);
+                        *reinterpret_cast<float4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(u.x, u.y, v.x, v.y);
                     }
                     __syncwarp();
-                    if (wide)
-                    {
-#pragma unroll
-                        for (int n = 0; n < 8; ++n)
-                        {
-                            const int q = n * 4 + (lane >> 3), j = lane & 7;
-                            if (first + q < a.rows)
-                                *reinterpret_cast<uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + j * VE) * SIZE) =
-                                    *reinterpret_cast<const uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4));
-                        }
-                    }
-                    else
-                        element_by_element<WIDE, SIZE>(a, out, first, k0 + c0, [&](int q, int c, char *there) {
-                            copy_element<SIZE>(there, stage + q * 128 + ((c / VE ^ (q & 7)) << 4) + c % VE * SIZE);
-                        });
+                    finish_rows<TYPE>(a, stage, first, k0 + c0 + 4 * (lane & 7), bias[c0 / 32]);
                     __syncwarp();
                 }
-            };
-            if (a.finish) // (asked for every value, a bias, an activation and old values took 0.7 us a tile that has none)
-                send(std::true_type());
-            else
-                send(std::false_type());
+                continue;
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < COLS; c0 += WIDE)
+            {
+                if (k0 + c0 >= a.K)
+                    break;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                {
+                    float v[VE];
+#pragma unroll
+                    for (int c = 0; c < VE; c += 2)
+                    {
+                        const float2 f = pair_of(acc[(c0 + j * VE + c) / 2]);
+                        v[c] = f.x;
+                        v[c + 1] = f.y;
+                    }
+                    uint4 w;
+                    if (TYPE == SMALL_B200_TYPE_F32)
+                        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                    else
+                        w = make_uint4(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]), pack2<TYPE>(v[VE - 4], v[VE - 3]),
+                                       pack2<TYPE>(v[VE - 2], v[VE - 1]));
+                    *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = w; // no two lanes of eight share banks
+                }
+                __syncwarp();
+                if (a.wide && k0 + c0 + WIDE <= a.K)
+                {
+#pragma unroll
+                    for (int n = 0; n < 8; ++n)
+                    {
+                        const int q = n * 4 + (lane >> 3), j = lane & 7;
+                        if (first + q < a.rows)
+                            *reinterpret_cast<uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + j * VE) * SIZE) =
+                                *reinterpret_cast<const uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4));
+                    }
+                }
+                else // element by element, a row at a time
+                {
+                    const int rows = min(32, a.rows - first);
+#pragma unroll 1
+                    for (int q = 0; q < rows; ++q)
+#pragma unroll
+                        for (int c = lane; c < WIDE; c += 32)
+                            if (k0 + c0 + c < a.K)
+                            {
+                                const uint8_t *src = stage + q * 128 + ((c / VE ^ (q & 7)) << 4) + c % VE * SIZE;
+                                char *dst = out + ((long long)(first + q) * a.out_stride + k0 + c0 + c) * SIZE;
+                                if (SIZE == 4)
+                                    *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
+                                else
+                                    *reinterpret_cast<uint16_t *>(dst) = *reinterpret_cast<const uint16_t *>(src);
+                            }
+                }
+                __syncwarp();
+            }
         }
     }
     else
