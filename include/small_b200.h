@@ -326,7 +326,7 @@ int small_b200_quantize_blocks_f8(int32_t rows, int32_t columns, int32_t block_r
                                   void *out, float *scales, void *stream);
 /* A dense layer on such operands (small::Dense, interface_abstract.hpp:2113, on 8-bit floats):
  *   out[r][k] = act(out[r][k] (accumulate) + bias[k] + sum over blocks b of in_scales[r][b] * filt_scales[k / 128][b] * dot of the block),
- * products and sums in fp32, one rounding to out_type at the end (with accumulate, after adding to what is there).
+ * products and sums in fp32, one rounding to out_type at the end (with accumulate, after adding to what is there); NaN stays NaN behind every activation.
  *   in    [rows][C] e4m3, scales [rows][ceil(C / 128)]          filt  [K][C] e4m3, scales [ceil(K / 128)][ceil(C / 128)]
  *   bias  [K] fp32 or NULL                                      out   [rows][K] of out_type
  * Strides are in elements between rows, 0 = packed; what lies between the K outputs of two rows is left as it is.  C % 16 == 0, in and filt on

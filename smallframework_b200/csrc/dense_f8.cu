@@ -7,8 +7,12 @@
 //
 // Two kernels:
 //   few    weights are the 128 lanes, 16, 32 or 64 rows of activations the columns.  The weights' bytes bound it: they come once, by TMA, into all SMs,
-//          the reduction cut among the CTAs of a cluster where output tiles are few; the parts are added over distributed shared memory, in order.
-//   many   128 rows of activations are the lanes, 256 outputs the columns.  The tensor cores bound it; one CTA an SM takes tile after tile.
+//          the reduction cut among the CTAs of a cluster where output tiles are few; the parts go to the CTA that finishes them by asynchronous stores and are
+//          added in order.  On a B200: 1 row, 4096 -> 4096 5.4 us (2.6 at the copy rate), 24 rows, 8192 -> 8192 15.3 (10.5): a microsecond until the first sums, one
+//          and a half for the exchange and the end, the launch; in between the weights come at 6.0 TB/s.
+//   many   256 rows of activations by 256 outputs for a pair of CTAs.  A block takes 975 cycles where its MMAs take 512: 32 KB an SM come from L2 at the device's
+//          10.4 TB/s in 840, and tensor memory holds two blocks' sums, whose way to the registers and back is 1400 cycles for the two.  From 4096 rows on the
+//          1 kW power cap (1.46 GHz) comes first.  2048 rows, 4096 -> 8192 69 us (1.99 PFLOP/s), with bias and ReLU 80; 8192, 8192 -> 8192 502 to 570 us.
 #include <algorithm>
 
 #include "narrow_types.cuh"

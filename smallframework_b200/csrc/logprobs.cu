@@ -10,8 +10,11 @@
 // Only these parts' vectors are read again, and only elements not below the last of the keys are ranked.  (Rows are read by so many CTAs at once that L2
 // does not hold them: with whole threads in place of quarters the second reading of 8 of 256 threads took 14 us of 107 at 2048 rows of 131072 classes.)
 //
-// Bound: memory, every logit read once.  A row is cut among the CTAs of a cluster where rows are few, and what they found is merged over distributed
-// shared memory (asynchronous stores to the first CTA): no workspace, and sums are always added in the same order.
+// Bound: memory, every logit read once, then the special-function pipe (62 % of its slots: an exponential a logit).  A row is cut among the CTAs of a cluster where
+// rows are few, and what they found is merged over distributed shared memory (asynchronous stores to the first CTA): no workspace, and sums are always added in
+// the same order.  Short rows, and longer ones where there are many, go to a warp each, which needs no barrier.
+// Measured on a B200: 2048x131072 bf16 with 8 alternatives 101 to 105 us (5.1 TB/s; 92 without alternatives; 83 at the copy rate), 6x131072 fp32 with 20
+// alternatives 11.4 us (12.6 where most classes are masked: equal logits are many candidates), 4096x1000 fp32 with 8 12.9 us, 1x1000 with 5 5.1 us.
 #include <algorithm>
 
 #include "narrow_types.cuh"
@@ -239,9 +242,9 @@ struct Shared
 };
 
 template <int TYPE, int WARPS>
-__global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_F32 ? 4 : 5) logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens,
-                                                            float *__restrict__ logprobs, float *__restrict__ entropy,
-                                                            float *__restrict__ top_logprobs, int *__restrict__ top_tokens, int *status)
+__global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_F32 ? 4 : 5)
+    logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens, float *__restrict__ logprobs,
+                    float *__restrict__ entropy, float *__restrict__ top_logprobs, int *__restrict__ top_tokens, int *status)
 {
     constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, BATCH = 4, THREADS = 32 * WARPS;
     constexpr int ROOM = sizeof(Shared<WARPS>::found) / 8;
@@ -714,7 +717,10 @@ extern "C" int small_b200_logprobs(int32_t rows, int32_t classes, int32_t in_typ
     if ((long long)rows * a.split > 0x7fffffffLL)
         return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: too many rows.");
     cudaStream_t st = as_stream(stream);
-    const bool narrow = a.split == 1 && classes <= 1024;
+    // A warp to a row or a CTA to a row, without and with 8 alternatives: 1 row of 500 fp32 classes 3.1/5.0 us and 2.8/5.8, of 1000 3.5/5.4 and 2.9/4.9; 300 rows of
+    // 700 3.5/5.4 and 4.0/10.2, of 2000 5.3/7.2 and 4.6/7.1; where the warps of all rows fill the SMs 1000 rows of 4000 7.6/10.0 and 10.4/14.7, of 8000 10.6/13.3 and
+    // 11.9/16.3, of 16000 28.1/32.0 and 18.9/23.5; 4096 rows of 4000 24/29 and 41/56; in bf16 1000 rows of 16000 12.7/16.7 and 12.7/18.2, of 32000 31.7/37.5 and 20.4/25.7.
+    const bool narrow = a.split == 1 && (classes <= 768 || (rows > 4 * num_sms() && (long long)classes * size <= 32768));
 #define SB_LOGP(T, W) launch_logprobs<T, W>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st)
     switch (in_type)
     {

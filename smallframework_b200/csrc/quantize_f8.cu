@@ -5,8 +5,10 @@
 // quotient.  A product with the rounded inverse is up to 2^-22 off, which matters only next to the middle between two codes (bf16 data meets
 // middles): both ends of that interval are converted, and only where the codes differ is x compared with middle * scale, exactly.
 //
-// Bound: memory (2 or 4 bytes read and one written an element).  16 lanes own 8 columns each of a block, so the largest magnitude of a row block is
-// four shuffles away and nothing is read twice.
+// Bound: memory (2 or 4 bytes read and one written an element), and close behind it the integer ALU (70 % of its slots at 8192x8192 bf16: unpacking, conversions,
+// packing).  16 lanes own 8 columns each of a block, so the largest magnitude of a row block is four shuffles away and nothing is read twice; four blocks a
+// lane are under way, and 16-bit values are compared two at a time as they are.
+// Measured on a B200: 8192x8192 bf16 40.5 us (5.0 TB/s, 31.2 at the copy rate), 5000x4112 fp32 in square blocks 20.7 us (5.0 TB/s, 15.9), 1x4096 2.0 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -148,18 +150,21 @@ struct Raw8
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 w[i] = has ? __ldg(q + i) : make_uint4(0u, 0u, 0u, 0u);
-            return;
         }
-        uint32_t v[4 * N];
+        else
+        {
+            uint32_t v[4 * N];
 #pragma unroll
-        for (int i = 0; i < 4 * N; ++i)
-            if (SIZE == 4)
-                v[i] = has ? __ldg(static_cast<const uint32_t *>(p) + at + i) : 0u;
-            else
-                v[i] = has ? __ldg(static_cast<const uint16_t *>(p) + at + 2 * i) | (uint32_t)__ldg(static_cast<const uint16_t *>(p) + at + 2 * i + 1) << 16 : 0u;
+            for (int i = 0; i < 4 * N; ++i)
+                if (SIZE == 4)
+                    v[i] = has ? __ldg(static_cast<const uint32_t *>(p) + at + i) : 0u;
+                else
+                    v[i] = has ? __ldg(static_cast<const uint16_t *>(p) + at + 2 * i) | (uint32_t)__ldg(static_cast<const uint16_t *>(p) + at + 2 * i + 1) << 16
+                               : 0u;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            w[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            for (int i = 0; i < N; ++i)
+                w[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
     }
     __device__ __forceinline__ void unpack(float *x) const
     {
