@@ -75,7 +75,8 @@ __device__ __forceinline__ uint8_t *align1024(uint8_t *p) { return p + ((1024u -
 template <int BN>
 struct Few
 {
-    // two CTAs an SM: 113 KB of shared memory and 256 columns of tensor memory each
+    // Two CTAs an SM: 113 KB of shared memory and 256 columns of tensor memory each.  Three never fit, so a launch that starts early cannot take tensor memory
+    // that a CTA of the launch before it, for which it waits, has yet to allocate.
     static constexpr int STAGE = A_BYTES + BN * KB, STAGES = BN == 16 ? 5 : BN == 32 ? 4 : 3;
     static constexpr int BUFS = 4, COLS = BUFS * BN;
     static constexpr int CHUNK = 8; // blocks whose scales are brought at a time
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
     cluster_arrive_relaxed(); // the barriers have been made and fenced
     cluster_wait();
     tc_fence_after_sync();
-    previous_kernel_done();
+    previous_kernel_done(); // tensor memory is this CTA's before the next launch may ask for it
     next_kernel_may_start();
     const uint32_t tmem = tmem_s;
 
