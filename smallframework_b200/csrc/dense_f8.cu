@@ -12,8 +12,9 @@
 //          and a half for the exchange and the end, the launch; in between the weights come at 6.0 TB/s.
 //   many   256 rows of activations by 256 outputs for a pair of CTAs.  A block takes 975 cycles where its MMAs take 512: 32 KB an SM come from L2 at the device's
 //          10.4 TB/s in 840, and tensor memory holds two blocks' sums, whose way to the registers and back is 1400 cycles for the two.  From 4096 rows on the
-//          1 kW power cap (1.46 GHz) comes first.  2048 rows, 4096 -> 8192 69 us (1.99 PFLOP/s), with bias and ReLU 80; 8192, 8192 -> 8192 502 to 570 us.
+//          1 kW power cap (1.46 GHz) comes first.  2048 rows, 4096 -> 8192 69 us (1.99 PFLOP/s), with bias and ReLU 71, onto old fp16 values 79; 8192, 8192 -> 8192 502 to 570 us.
 #include <algorithm>
+#include <type_traits>
 
 #include "narrow_types.cuh"
 #include "tc_common.cuh"
@@ -35,7 +36,6 @@ struct DenseArgs
     long long out_stride;
     const float *in_scales, *filt_scales, *bias;
     void *out;
-    int finish; // a bias, an activation or an old value
     int wide; // rows of the output begin on 16-byte boundaries
 };
 
@@ -66,6 +66,37 @@ __device__ __forceinline__ void fold2(unsigned long long &acc, uint32_t lo, uint
     unsigned long long r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(r), "l"(s2));
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b)
+{
+    unsigned long long v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+// Four bytes into shared memory, past the registers; copies_done() waits for this thread's.
+__device__ __forceinline__ void copy4(void *to, const float *from)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ unsigned long long activate2(unsigned long long v, bool relu, float below)
+{
+    float x, y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+    x = activate(x, relu, below);
+    y = activate(y, relu, below);
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+// The two 16-bit floats of a word.
+template <int TYPE>
+__device__ __forceinline__ unsigned long long wide2(uint32_t w)
+{
+    float x, y;
+    unsigned long long v;
+    unpack2<TYPE>(w, x, y);
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
 }
 __device__ __forceinline__ float2 pair_of(unsigned long long v) { return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))); }
 
@@ -494,38 +525,55 @@ __device__ __forceinline__ void fold32(unsigned long long *acc, const uint32_t *
         fold2(acc[c], r[2 * c], r[2 * c + 1], s2);
 }
 
-// Eight of a warp's 32 rows, four columns from k on, out of its shared memory.  In line and in a loop: a call keeps what it saves, and long code what does not
-// fit, in local memory, which beside 227 KB of shared memory is hardly cached (8 us a tile).
-template <int TYPE>
-__device__ __forceinline__ void finish_rows(const DenseArgs &a, const uint8_t *stage, int first, int k, float4 bias)
+// A warp's copy of the bias of its COLS outputs.
+template <int COLS>
+__device__ __forceinline__ void copy_bias(const DenseArgs &a, uint8_t *to, int k0)
 {
     const int lane = threadIdx.x & 31;
-    if (k >= a.K)
-        return;
-    constexpr int TOGETHER = 2; // short code: what a tile runs through once has to be fetched, 4 us a launch with four at a time
-    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32)
+        copy4(to + (c + lane) * 4, a.bias + min(k0 + c + lane, a.K - 1));
+}
+// 128 bytes of each of a warp's 32 rows, from output k on, between the output and the warp's shared memory (OUT: to the output): element by element, a row at a
+// time on the way out, as many together on the way in as hide that a load takes its time.
+template <int TYPE, bool OUT>
+__device__ __forceinline__ void by_element(const DenseArgs &a, uint8_t *stage, int first, int k)
+{
+    using Word = typename std::conditional<TYPE == SMALL_B200_TYPE_F32, uint32_t, uint16_t>::type;
+    constexpr int VE = 16 / sizeof(Word), EACH = 8 * VE / 32, TOGETHER = OUT ? 1 : 8;
+    const int lane = threadIdx.x & 31, rows = min(32, a.rows - first);
+    Word *out = static_cast<Word *>(a.out) + (long long)first * a.out_stride + k;
 #pragma unroll 1
-    for (int at = 0; at < 8; at += TOGETHER)
+    for (int q0 = 0; q0 < rows; q0 += TOGETHER)
     {
-        float4 old[TOGETHER];
-        int row[TOGETHER];
+        Word old[TOGETHER][EACH];
 #pragma unroll
         for (int n = 0; n < TOGETHER; ++n)
-        {
-            row[n] = (lane >> 3) + 4 * (at + n);
-            old[n] = a.accumulate && first + row[n] < a.rows ? load4<TYPE>(a, first + row[n], k) : none;
-        }
 #pragma unroll
-        for (int n = 0; n < TOGETHER; ++n)
-        {
-            const float4 sum = *reinterpret_cast<const float4 *>(stage + row[n] * 128 + (((lane & 7) ^ (row[n] & 7)) << 4));
-            if (first + row[n] < a.rows)
-                store4<TYPE>(a, first + row[n], k, finished(a, sum, old[n], bias));
-        }
+            for (int e = 0; e < EACH; ++e)
+            {
+                const int q = q0 + n, c = lane + 32 * e;
+                const bool has = q < rows && k + c < a.K;
+                Word *in = reinterpret_cast<Word *>(stage + q * 128 + ((c / VE ^ (q & 7)) << 4)) + c % VE;
+                if (OUT && has)
+                    out[q * a.out_stride + c] = *in;
+                else if (!OUT)
+                    old[n][e] = has ? out[q * a.out_stride + c] : (Word)0;
+            }
+        if (!OUT)
+#pragma unroll
+            for (int n = 0; n < TOGETHER; ++n)
+#pragma unroll
+                for (int e = 0; e < EACH; ++e)
+                {
+                    const int q = q0 + n, c = lane + 32 * e;
+                    *(reinterpret_cast<Word *>(stage + q * 128 + ((c / VE ^ (q & 7)) << 4)) + c % VE) = old[n][e];
+                }
     }
 }
 
-template <int TYPE, int N>
+// FINISH: with a bias, an activation or old values; code that a tile jumps over costs it 0.3 us.
+template <int TYPE, int N, bool FINISH>
 __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                           const DenseArgs a, int *status)
 {
@@ -578,6 +626,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                 acc[c] = 0ull;
             // Software pipeline over the blocks: while 32 columns are folded the next 32 are on their way, across blocks too, and the next block's
             // barrier is asked one step before its answer is needed.
+            if (FINISH && a.bias && !a.accumulate) // asked for now, needed at the end, and until then not in registers
+                copy_bias<COLS>(a, ring + MANY_STAGES * MANY_STAGE + (warp - 4) * STAGE_OUT, k0);
             float next_x = __ldg(sx), next_w = __ldg(sw); // multiplied when they are needed: until then nothing waits for them
             uint32_t r[2][32];
             ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[i % BUFS], (i / BUFS) & 1, status, 111));
@@ -636,30 +686,81 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             uint8_t *stage = ring + MANY_STAGES * MANY_STAGE + (warp - 4) * STAGE_OUT;
             const int first = at.r0 + rank * 128 + (warp & 3) * 32; // row of the warp
             char *out = static_cast<char *>(a.out);
-            if (a.finish)
+            if (FINISH && a.accumulate)
             {
-                // With a bias, an activation or old values: the sums go in as they are, 32 columns at a time, and a lane finishes four columns of eight
-                // rows.  (Every thread by itself for its row's bias was 5 us a tile.)
-                float4 bias[COLS / 32];
+                // The old values, the same way in: whole lines of four rows, then every thread its row's.
 #pragma unroll
-                for (int c0 = 0; c0 < COLS; c0 += 32)
-                    bias[c0 / 32] = bias4(a, k0 + c0 + 4 * (lane & 7));
-#pragma unroll
-                for (int c0 = 0; c0 < COLS; c0 += 32)
+                for (int c0 = 0; c0 < COLS; c0 += WIDE)
                 {
                     if (k0 + c0 >= a.K)
                         break;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                    if (a.wide && k0 + c0 + WIDE <= a.K)
                     {
-                        const float2 u = pair_of(acc[c0 / 2 + 2 * j]), v = pair_of(acc[c0 / 2 + 2 * j + 1]);
-                        *reinterpret_cast<float4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(u.x, u.y, v.x, v.y);
+                        uint4 old[8];
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+                        {
+                            const int q = n * 4 + (lane >> 3);
+                            if (first + q < a.rows)
+                                old[n] = *reinterpret_cast<const uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + (lane & 7) * VE) * SIZE);
+                            else
+                                old[n] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+                            *reinterpret_cast<uint4 *>(stage + (n * 4 + (lane >> 3)) * 128 + (((lane & 7) ^ (n * 4 + (lane >> 3) & 7)) << 4)) = old[n];
+                    }
+                    else
+                        by_element<TYPE, false>(a, stage, first, k0 + c0);
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) // what lies behind the last row or output is added to sums that go nowhere
+                    {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4));
+                        unsigned long long *to = acc + (c0 + j * VE) / 2;
+                        if (TYPE == SMALL_B200_TYPE_F32)
+                        {
+                            to[0] = add2(to[0], (unsigned long long)w.y << 32 | w.x);
+                            to[1] = add2(to[1], (unsigned long long)w.w << 32 | w.z);
+                        }
+                        else
+                        {
+                            to[0] = add2(to[0], wide2<TYPE>(w.x));
+                            to[1] = add2(to[1], wide2<TYPE>(w.y));
+                            to[VE / 2 - 2] = add2(to[VE / 2 - 2], wide2<TYPE>(w.z));
+                            to[VE / 2 - 1] = add2(to[VE / 2 - 1], wide2<TYPE>(w.w));
+                        }
                     }
                     __syncwarp();
-                    finish_rows<TYPE>(a, stage, first, k0 + c0 + 4 * (lane & 7), bias[c0 / 32]);
-                    __syncwarp();
                 }
-                continue;
+                if (a.bias)
+                    copy_bias<COLS>(a, stage, k0);
+            }
+            if (FINISH && a.bias)
+            {
+                // Every thread needs the same numbers: a copy in the warp's way out serves a whole warp a load.  (Loads from global memory were 5 us a tile.)
+                copies_done();
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < COLS; c += 4)
+                {
+                    const ulonglong2 b = reinterpret_cast<const ulonglong2 *>(stage)[c / 4];
+                    acc[c / 2] = add2(acc[c / 2], b.x);
+                    acc[c / 2 + 1] = add2(acc[c / 2 + 1], b.y);
+                }
+                __syncwarp();
+            }
+            if (FINISH && a.act == SMALL_B200_ACT_RELU)
+            {
+#pragma unroll
+                for (int c = 0; c < COLS / 2; ++c)
+                    acc[c] = activate2(acc[c], true, 1.f);
+            }
+            else if (FINISH && a.act == SMALL_B200_ACT_LEAKY)
+            {
+#pragma unroll
+                for (int c = 0; c < COLS / 2; ++c)
+                    acc[c] = activate2(acc[c], false, a.slope);
             }
 #pragma unroll
             for (int c0 = 0; c0 < COLS; c0 += WIDE)
@@ -697,26 +798,13 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                                 *reinterpret_cast<const uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4));
                     }
                 }
-                else // element by element, a row at a time
-                {
-                    const int rows = min(32, a.rows - first);
-#pragma unroll 1
-                    for (int q = 0; q < rows; ++q)
-#pragma unroll
-                        for (int c = lane; c < WIDE; c += 32)
-                            if (k0 + c0 + c < a.K)
-                            {
-                                const uint8_t *src = stage + q * 128 + ((c / VE ^ (q & 7)) << 4) + c % VE * SIZE;
-                                char *dst = out + ((long long)(first + q) * a.out_stride + k0 + c0 + c) * SIZE;
-                                if (SIZE == 4)
-                                    *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
-                                else
-                                    *reinterpret_cast<uint16_t *>(dst) = *reinterpret_cast<const uint16_t *>(src);
-                            }
-                }
+                else
+                    by_element<TYPE, true>(a, stage, first, k0 + c0);
                 __syncwarp();
             }
         }
+        if (FINISH)
+            copies_done(); // also where a wait gave up
     }
     else
     {
@@ -853,10 +941,10 @@ int launch_few(DenseArgs a, const CUtensorMap &map_w, const CUtensorMap &map_x, 
     return launched("dense_f8_few_kernel");
 }
 
-template <int TYPE, int N>
+template <int TYPE, int N, bool FINISH>
 int launch_many(const DenseArgs &a, const CUtensorMap &map_x, const CUtensorMap &map_w, int *status, cudaStream_t st)
 {
-    auto kern = dense_f8_many_kernel<TYPE, N>;
+    auto kern = dense_f8_many_kernel<TYPE, N, FINISH>;
     static PerDeviceOnce configured;
     int dev;
     if (configured.needed(&dev))
@@ -913,6 +1001,7 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
         default: return launch_few<64, TYPE>(a, map_w, map_x, status, st);
         }
     }
+    const bool finish = a.bias || a.accumulate || a.act != SMALL_B200_ACT_NONE;
     a.k_tiles = (D->K + 255) / 256;
     a.r_tiles = (D->rows + 255) / 256;
     a.split = 1;
@@ -924,7 +1013,7 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
             return rc;
         a.first = 0;
         a.count = (int)(halves ? whole : pairs_of_tiles);
-        if (int rc = launch_many<TYPE, 256>(a, map_x, map_w, status, st))
+        if (int rc = finish ? launch_many<TYPE, 256, true>(a, map_x, map_w, status, st) : launch_many<TYPE, 256, false>(a, map_x, map_w, status, st))
             return rc;
     }
     if (!halves)
@@ -933,7 +1022,7 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
         return rc;
     a.first = (int)whole;
     a.count = (int)rest;
-    return launch_many<TYPE, 128>(a, map_x, map_w, status, st);
+    return finish ? launch_many<TYPE, 128, true>(a, map_x, map_w, status, st) : launch_many<TYPE, 128, false>(a, map_x, map_w, status, st);
 }
 } // namespace
 
@@ -970,7 +1059,6 @@ extern "C" int small_b200_dense_f8(const small_b200_dense *D, const void *in, co
     a.rows = D->rows; a.K = D->K; a.blocks = (D->C + KB - 1) / KB;
     a.accumulate = D->accumulate; a.act = D->act; a.slope = D->slope;
     a.out_stride = out_stride; a.in_scales = in_scales; a.filt_scales = filt_scales; a.bias = bias; a.out = out;
-    a.finish = bias || D->accumulate || D->act != SMALL_B200_ACT_NONE;
     a.wide = !off(out, 16) && out_stride * size % 16 == 0;
     cudaStream_t st = as_stream(stream);
     switch (D->out_type)
