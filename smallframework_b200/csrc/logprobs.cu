@@ -14,7 +14,7 @@
 // rows are few, and what they found is merged over distributed shared memory (asynchronous stores to the first CTA): no workspace, and sums are always added in
 // the same order.  Short rows, and longer ones where there are many, go to a warp each, which needs no barrier.
 // Measured on a B200: 2048x131072 bf16 with 8 alternatives 101 to 105 us (5.1 TB/s; 92 without alternatives; 83 at the copy rate), 6x131072 fp32 with 20
-// alternatives 11.4 us (12.6 where most classes are masked: equal logits are many candidates), 4096x1000 fp32 with 8 12.9 us, 1x1000 with 5 5.1 us.
+// alternatives 10.0 us (11.0 where rows are masked), 160x50257 fp16 with 10 12.2, 4096x1000 fp32 with 8 12.9 us, 1x1000 with 5 5.1 us.
 #include <algorithm>
 
 #include "narrow_types.cuh"
@@ -226,18 +226,67 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long key, 
     return key;
 }
 
+// How many of a list's keys are above `k`.
+__device__ __forceinline__ int rank_in(const unsigned long long *list, int n, unsigned long long k)
+{
+    int before = 0;
+#pragma unroll 4
+    for (int q = 0; q + 1 < n; q += 2)
+    {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(list + q);
+        before += (two.x > k) + (two.y > k);
+    }
+    return before + ((n & 1) && list[n - 1] > k);
+}
+constexpr int SHORT = 96; // lists that are ranked as they are: 160 rows of 50257 fp16, some masked whole, 20 alternatives 13.3 us for 64 and 96, 13.8 for 32, 16.9 for all lists
+// Leaves in a long list (at most CANDIDATES keys, none 0) those that reach a bound which `top` of them reach, and returns how many: ranking takes the square of a
+// list's length.  As for the parts' bound each warp's ceil(top / 8) th best is asked for; neighbours in the list, which came from one warp, go to different ones.
+// By all threads; `count` is 0 and used for nothing else.  One copy of the code for all lists.
+__device__ __noinline__ int keep_best(unsigned long long *list, int n, int top, unsigned long long *bounds, int *count)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned long long key[CANDIDATES / 256], mine = 0ull, nth = 0ull;
+#pragma unroll
+    for (int j = 0; j < CANDIDATES / 256; ++j)
+    {
+        const int i = j * 256 + lane * 8 + warp;
+        key[j] = i < n ? list[i] : 0ull;
+        mine = key[j] > mine ? key[j] : mine;
+    }
+    for (int i = 0; i < (top + 7) / 8; ++i)
+    {
+        const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
+        const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32) == high ? (uint32_t)mine : 0u);
+        nth = (unsigned long long)high << 32 | low;
+        mine = mine == nth ? 0ull : mine;
+    }
+    if (lane == 0)
+        bounds[warp] = nth;
+    __syncthreads(); // the list has been read
+    unsigned long long bound = bounds[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w)
+        bound = bounds[w] < bound ? bounds[w] : bound;
+#pragma unroll
+    for (int j = 0; j < CANDIDATES / 256; ++j)
+        if (key[j] != 0ull && key[j] >= bound)
+            list[atomicAdd(count, 1)] = key[j];
+    __syncthreads();
+    return *count;
+}
+
 template <int WARPS>
 struct Shared
 {
     Stats part[WARPS], all;
     unsigned long long bound[WARPS], last;
     unsigned long long best[TOP_MOST]; // this CTA's best elements, in order
-    unsigned long long found[WARPS == 1 ? 256 : CANDIDATES];
+    alignas(16) unsigned long long found[WARPS == 1 ? 256 : CANDIDATES];
     unsigned long long keys[PARTS * 32 * WARPS];
-    unsigned long long merged[WARPS == 1 ? 1 : MAX_SPLIT * TOP_MOST];
+    alignas(16) unsigned long long merged[WARPS == 1 ? 2 : MAX_SPLIT * TOP_MOST];
     float4 of_cta[MAX_SPLIT]; // every CTA's maximum and sums, in the first
     int first[TOP_MOST];      // the best parts' first vectors
-    int count;
+    int parts, parts_kept, candidates, candidates_kept; // how many are in the lists
     uint64_t delivered;
 };
 
@@ -432,7 +481,7 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
     if (lane == 0)
         sh.part[warp] = st;
     if (tid == 0)
-        sh.count = 0;
+        sh.parts = sh.parts_kept = sh.candidates = sh.candidates_kept = 0;
 
     if (a.top > 0)
     {
@@ -470,16 +519,15 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
 #pragma unroll
         for (int q = 0; q < PARTS; ++q)
             if (key[q] != 0ull && key[q] >= bound)
-                sh.found[atomicAdd(&sh.count, 1)] = key[q];
+                sh.found[atomicAdd(&sh.parts, 1)] = key[q];
         sync_row<WARPS>();
-        const int reach = sh.count;
+        int reach = sh.parts;
+        if (WARPS > 1 && reach > SHORT) // equal logits: the first warp's parts are all before the next one's
+            reach = keep_best(sh.found, reach, a.top, sh.bound, &sh.parts_kept);
         for (int i = tid; i < reach; i += THREADS)
         {
             const unsigned long long k = sh.found[i];
-            int before = 0;
-#pragma unroll 4
-            for (int q = 0; q < reach; ++q)
-                before += sh.found[q] > k;
+            const int before = rank_in(sh.found, reach, k);
             if (before < a.top)
             {
                 const int steps_in = (int)(0xffffffffu - (uint32_t)k - (uint32_t)v0) / THREADS, thread = (int)(0xffffffffu - (uint32_t)k - (uint32_t)v0) % THREADS;
@@ -488,9 +536,6 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
             if (before == a.top - 1)
                 sh.last = k;
         }
-        sync_row<WARPS>();
-        if (tid == 0)
-            sh.count = 0;
         sync_row<WARPS>();
         // ---- their elements that are not below the last of them
         const int best_parts = min(reach, a.top);
@@ -533,21 +578,20 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
             }
         };
         each([&](unsigned long long k) {
-            const int n = atomicAdd(&sh.count, 1);
+            const int n = atomicAdd(&sh.candidates, 1);
             if (n < ROOM)
                 sh.found[n] = k;
         });
         sync_row<WARPS>();
-        const int n = sh.count;
+        int n = sh.candidates;
         if (n <= ROOM)
         {
+            if (WARPS > 1 && n > SHORT)
+                n = keep_best(sh.found, n, a.top, sh.bound, &sh.candidates_kept);
             for (int i = tid; i < n; i += THREADS)
             {
                 const unsigned long long k = sh.found[i];
-                int before = 0;
-#pragma unroll 4
-                for (int q = 0; q < n; ++q)
-                    before += sh.found[q] > k;
+                const int before = rank_in(sh.found, n, k);
                 if (before < a.top)
                     sh.best[before] = k;
             }
@@ -628,10 +672,7 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
             for (int i = tid; i < n; i += THREADS)
             {
                 const unsigned long long k = sh.merged[i];
-                int before = 0;
-#pragma unroll 4
-                for (int q = 0; q < n; ++q)
-                    before += sh.merged[q] > k;
+                const int before = rank_in(sh.merged, n, k);
                 if (k != 0ull && before < a.top)
                     sh.found[before] = k;
             }
@@ -710,9 +751,14 @@ extern "C" int small_b200_logprobs(int32_t rows, int32_t classes, int32_t in_typ
         return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: misaligned buffer.");
     LogpArgs a;
     a.rows = rows; a.stride = stride ? stride : classes; a.classes = classes; a.top = top; a.token_bytes = token_bytes;
-    // As many CTAs to a row as are resident at once, while each of their threads has a vector of its own.
+    // CTAs to a row, while each of their threads has a vector of its own.  What a CTA does besides reading (the best alternatives, the cluster) is 4 to 5 us, so more
+    // of them than two an SM pay only for rows of 256 KB on, and eight a row only for few of such rows.  With 8 alternatives, one, two and four CTAs a row:
+    // 160 rows of 131072 fp32 classes 34.3, 25.4 and 30.4 us, of 50257 fp16 11.1, 11.2, 13.7; 148 rows of 50257 9.9, 9.7, 12.4; 592 of 131072 fp32 52.5, 60.6, 78.3.
+    // Four and eight: 6 rows of 131072 fp32 9.8 and 8.6, of 50257 fp16 8.3 and 8.8.
+    const bool longer = (long long)classes * size >= 256 << 10;
     a.split = 1;
-    while (a.split < MAX_SPLIT && (long long)rows * a.split * 2 <= 4LL * num_sms() && classes / (16 / size) >= 2 * a.split * 256)
+    while (a.split < (longer ? MAX_SPLIT : MAX_SPLIT / 2) && rows * 2LL * a.split <= (a.split == 1 && longer ? 4LL : a.split < 4 ? 2LL : 1LL) * num_sms() &&
+           classes / (16 / size) >= 2 * a.split * 256)
         a.split *= 2;
     if ((long long)rows * a.split > 0x7fffffffLL)
         return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: too many rows.");
