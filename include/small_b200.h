@@ -321,7 +321,7 @@ enum
  *   in      rows of in_type, in_stride elements apart (0 = packed)
  *   out     [rows][columns] bytes, on a 16-byte boundary
  *   scales  [rows or ceil(rows / 128)][ceil(columns / 128)]
- * columns % 16 == 0; fewer than 2^31 blocks. */
+ * columns % 16 == 0; fewer than 2^31 blocks; in and out are different memory. */
 int small_b200_quantize_blocks_f8(int32_t rows, int32_t columns, int32_t block_rows, int32_t in_type, const void *in, int64_t in_stride,
                                   void *out, float *scales, void *stream);
 /* A dense layer on such operands (small::Dense, interface_abstract.hpp:2113, on 8-bit floats):
@@ -330,7 +330,8 @@ int small_b200_quantize_blocks_f8(int32_t rows, int32_t columns, int32_t block_r
  *   in    [rows][C] e4m3, scales [rows][ceil(C / 128)]          filt  [K][C] e4m3, scales [ceil(K / 128)][ceil(C / 128)]
  *   bias  [K] fp32 or NULL                                      out   [rows][K] of out_type
  * Strides are in elements between rows, 0 = packed; what lies between the K outputs of two rows is left as it is.  C % 16 == 0, in and filt on
- * 16-byte boundaries with strides that are multiples of 16.  The product of two scales is rounded to fp32, so it should be a normal number. */
+ * 16-byte boundaries with strides that are multiples of 16.  The product of two scales is rounded to fp32, so it should be a normal number.
+ * rows, K and C up to 2^31 - 513; out is memory of its own. */
 typedef struct small_b200_dense
 {
     int32_t rows, K, C;

@@ -1053,7 +1053,8 @@ extern "C" int small_b200_dense_f8(const small_b200_dense *D, const void *in, co
     auto off = [](const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
     if (off(in, 16) || off(filt, 16) || off(in_scales, 4) || off(filt_scales, 4) || off(bias, 4) || off(out, size))
         return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: misaligned buffer (operands begin on 16-byte boundaries).");
-    if (((D->K + 127LL) / 128) * ((D->rows + 15LL) / 16) * 8 > 0x7fffffffLL)
+    constexpr int MOST = 0x7fffffff - 512; // a tile behind the last row or output is still an int
+    if (D->rows > MOST || D->K > MOST || D->C > MOST || ((D->K + 127LL) / 128) * ((D->rows + 15LL) / 16) * 8 > 0x7fffffffLL)
         return fail(SMALL_B200_INVALID_ARGUMENT, name + " ERROR: too many tiles.");
     DenseArgs a = {};
     a.rows = D->rows; a.K = D->K; a.blocks = (D->C + KB - 1) / KB;

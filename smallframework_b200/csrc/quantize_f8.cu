@@ -369,7 +369,7 @@ extern "C" int small_b200_quantize_blocks_f8(int32_t rows, int32_t columns, int3
     if (reinterpret_cast<uintptr_t>(in) % size != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 4 != 0)
         return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: misaligned buffer (the codes begin on a 16-byte boundary).");
     QuantArgs a;
-    a.rows = rows; a.columns = columns; a.blocks = (columns + 127) / 128;
+    a.rows = rows; a.columns = columns; a.blocks = (int)((columns + 127LL) / 128);
     a.stride = in_stride ? in_stride : columns;
     a.units = (long long)(block_rows == 1 ? rows : (rows + 127LL) / 128) * a.blocks;
     if (a.units > 0x7fffffffLL)
