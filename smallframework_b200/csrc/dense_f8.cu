@@ -969,26 +969,29 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
     if (!status)
         return fail(SMALL_B200_CUDA_ERROR, "device status word not available");
     CUtensorMap map_w, map_x;
-    // Microseconds that either kernel takes, fitted to 91 sizes (1 to 2048 rows, 512 to 8192 outputs and inputs): a tile and block of 128 outputs by 64 rows
-    // costs the device 3.1 ns in the one, a block of a wave of 256 x 256 tiles 0.48 us in the other, of halves of such tiles 0.27.
-    // 256 rows, 8192 -> 1024: 12.1 and 23.0 us; 256 rows, 4096 -> 4096: 16.4 and 14.2; 128 rows: 11.0 and 14.0; 1024 rows, 8192 -> 1024: 24.9 and 23.7.
-    const double units = (double)((D->K + 127LL) / 128) * ((D->rows + 63LL) / 64) * a.blocks;
+    // Microseconds that either kernel takes, fitted to 136 sizes of 64 to 512 rows, 64 to 8192 outputs and 512 to 8192 inputs (on average 0.2 % are lost against the
+    // faster one): a start and an end, a tile of 128 outputs by 64 rows and its blocks in the one, a wave of 256 x 256 tiles, or of halves of such tiles, in the
+    // other.  64 rows, 512 -> 4096: 5.6 us and 4.7; 128 rows, 4096 -> 4096: 10.9 and 12.9; 256 rows: 15.5 and 13.2; 512 rows, 8192 -> 1024: 15.1 and 21.9.
+    const double b = a.blocks, tiles_of_few = (double)((D->K + 127LL) / 128) * ((D->rows + 63LL) / 64);
     const long long pairs_of_tiles = ((D->K + 255LL) / 256) * ((D->rows + 255LL) / 256), at_once = std::max(1, num_sms() / 2);
-    // Tiles for which there are twice as many pairs of CTAs are done in halves, a launch of its own behind whole waves (2.5 us).
+    // Tiles for which there are twice as many pairs of CTAs are done in halves, a launch of its own behind whole waves.
     const long long whole = pairs_of_tiles / at_once * at_once, rest = pairs_of_tiles - whole;
     const bool halves = rest > 0 && 2 * rest <= at_once;
-    const double few_us = 4.5 + 0.0031 * units;
-    const double many_us = 4.5 + (double)(whole / at_once) * (0.48 * a.blocks + 1.5) +
-                           (rest == 0 ? 0. : halves ? 0.27 * a.blocks + 1. + (whole > 0 ? 2.5 : 0.) : 0.48 * a.blocks + 1.5);
-    if (D->rows <= 64 || few_us < many_us)
+    const double few_us = 4.7 + 0.048 * b + tiles_of_few * (0.0095 + 0.00203 * b), wave = 0.47 * b + 1.9;
+    const double many_us = 3.2 + (double)(whole / at_once) * wave + (rest == 0 ? 0. : halves ? 0.285 * b + (whole > 0 ? 3.2 : 0.) : wave);
+    if (D->rows <= 32 || few_us < many_us)
     {
         const int bn = D->rows <= 16 ? 16 : D->rows <= 32 ? 32 : 64;
         a.k_tiles = (D->K + 127) / 128;
         a.r_tiles = (D->rows + bn - 1) / bn;
-        // Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each at least two blocks.  Clusters of eight come up slowly
-        // (the last of 32 after 1.8 us, of 64 clusters of four after 0.9): only where four leave SMs without a CTA.
+        // Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each at least two blocks.  Clusters of four and eight do not fill every
+        // group of SMs (148 SMs hold 70 and 33): 1 row, 4096 inputs, 70 tiles of outputs 9.0 us in fours and 9.9 in twos, but 72 tiles 13.4 and 10.0; 8192 inputs,
+        // 33 tiles 8.0 in eights and 8.8 in fours, but 34 tiles 12.2 and 10.1.  Clusters of eight come up slowly (the last of 32 after 1.8 us, of 64 clusters of four
+        // after 0.9), so short reductions are cut in eight only where four leave SMs without a CTA: 64 rows, 2048 inputs, 20 tiles 7.2 and 6.8, 15 tiles 5.5 and 6.5.
+        const long long tiles = (long long)a.k_tiles * a.r_tiles, sms = num_sms();
         a.split = 1;
-        while (a.split < 8 && (long long)a.k_tiles * a.r_tiles * a.split * 2 <= (a.split < 4 ? 2LL : 1LL) * num_sms() && a.blocks >= 4 * a.split)
+        while (a.split < 8 && a.blocks >= 4 * a.split &&
+               tiles * 2 * a.split <= (a.split == 1 ? 2 * sms : a.split == 2 ? 2 * sms - 16 : a.blocks >= 32 ? 2 * sms - 32 : sms))
             a.split *= 2;
         if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, 128))
             return rc;

@@ -733,7 +733,7 @@ def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, o
     _size(name, C_)
     apart = K if out_stride is None else out_stride
     # (a slope of -0.0 is another one than 0.0, but not another key)
-    L = (_dense_layer if slope else _dense_layer.__wrapped__)(rows, K, C_, _TYPES[y.dtype], apart, accumulate, act, slope)
+    L = (_dense_layer if slope or math.copysign(1.0, slope) > 0 else _dense_layer.__wrapped__)(rows, K, C_, _TYPES[y.dtype], apart, accumulate, act, slope)
     blocks, here = -(-C_ // 128), _home(name, y, "output")
     elems = (rows - 1) * apart + K if rows > 0 else 0
     x, xs, w, ws = inp.t, inp.scales, filt.t, filt.scales
