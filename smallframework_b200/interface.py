@@ -687,6 +687,15 @@ def _size(name, n):
         raise ValueError(f"{name}: a size of {n}")
 
 
+def _stride(name, columns, apart):
+    """Elements between rows.  (0 means packed to the library, so a count of elements must not be made with it.)"""
+    if apart is None:
+        return columns
+    if not columns <= apart < 1 << 63:
+        raise ValueError(f"{name}: rows of {columns} elements that are {apart} apart")
+    return apart
+
+
 _F32, _F8, _I32, _TOKENS = torch.float32, torch.float8_e4m3fn, torch.int32, (torch.int32, torch.int64)
 _FLOATS = tuple(_TYPES)
 
@@ -702,7 +711,7 @@ def QuantizeBlocks(num_rows, num_columns, input_buf, output_buf, *, input_stride
         raise ValueError(f"{name}: an output of {output_buf.rows} x {output_buf.columns} for {num_rows} x {num_columns}")
     _size(name, num_rows)
     _size(name, num_columns)
-    apart = num_columns if input_stride is None else input_stride
+    apart = _stride(name, num_columns, input_stride)
     x = _tensor(input_buf)
     here = _home(name, x, "input")
     q, scales, m = output_buf.t, output_buf.scales, output_buf.block_rows
@@ -731,7 +740,7 @@ def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, o
     _size(name, rows)
     _size(name, K)
     _size(name, C_)
-    apart = K if out_stride is None else out_stride
+    apart = _stride(name, K, out_stride)
     # (a slope of -0.0 is another one than 0.0, but not another key)
     L = (_dense_layer if slope or math.copysign(1.0, slope) > 0 else _dense_layer.__wrapped__)(rows, K, C_, _TYPES[y.dtype], apart, accumulate, act, slope)
     blocks, here = -(-C_ // 128), _home(name, y, "output")
@@ -772,7 +781,7 @@ def LogProbabilities(num_rows, num_classes, logits_buf, tokens, logprobs_buf, en
     _size(name, num_rows)
     _size(name, num_classes)
     _size(name, top)
-    apart = num_classes if row_stride is None else row_stride
+    apart = _stride(name, num_classes, row_stride)
     x = _tensor(logits_buf)
     here = _home(name, x, "logits")
     elems, each = (num_rows - 1) * apart + num_classes if num_rows > 0 else 0, num_rows * top
