@@ -651,12 +651,16 @@ def Conv2D_ReLU_DepthwiseConv2D_ReLU(conv_kernel_height, conv_kernel_width, conv
 
 
 # --------------------------------------------------------------------------- narrow types
+_device_now = _device or torch.cuda.current_device
+_stream_now = _raw_stream or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _home(name, t, what):
     """The current device's number, which is the tensor's too."""
     here = t.get_device()
     if here < 0:
         raise _lib.SmallB200Error("buffers must live on a CUDA device (no CPU path)")
-    now = _device() if _device is not None else torch.cuda.current_device()
+    now = _device_now()
     if here != now:
         raise ValueError(f"{name}: {what} on cuda:{here}, the current device is cuda:{now}")
     return here
@@ -682,9 +686,13 @@ def _tensor(buf):
     return buf if isinstance(buf, torch.Tensor) else buf.t
 
 
-def _size(name, n):
-    if not 0 <= n < 1 << 31:  # a longer one would lose its upper bits on the way to the library
-        raise ValueError(f"{name}: a size of {n}")
+_MOST = 1 << 31  # a larger size would lose its upper bits on the way to the library
+
+
+def _sizes(name, *sizes):
+    for n in sizes:
+        if not 0 <= n < _MOST:
+            raise ValueError(f"{name}: a size of {n}")
 
 
 def _stride(name, columns, apart):
@@ -707,24 +715,28 @@ def QuantizeBlocks(num_rows, num_columns, input_buf, output_buf, *, input_stride
     name = "QuantizeBlocks"
     if not isinstance(output_buf, Float8Buffer):
         raise ValueError(f"{name}: the output is a Float8Buffer")
-    if (output_buf.rows, output_buf.columns) != (num_rows, num_columns):
+    if output_buf.rows != num_rows or output_buf.columns != num_columns:
         raise ValueError(f"{name}: an output of {output_buf.rows} x {output_buf.columns} for {num_rows} x {num_columns}")
-    _size(name, num_rows)
-    _size(name, num_columns)
-    apart = _stride(name, num_columns, input_stride)
-    x = _tensor(input_buf)
-    here = _home(name, x, "input")
+    if not (0 <= num_rows < _MOST and 0 <= num_columns < _MOST):
+        _sizes(name, num_rows, num_columns)
+    apart = num_columns if input_stride is None else _stride(name, num_columns, input_stride)
+    x = input_buf if isinstance(input_buf, torch.Tensor) else input_buf.t
+    kind, here = _TYPES.get(x.dtype), x.get_device()
+    if here < 0 or here != _device_now():
+        _home(name, x, "input")
     q, scales, m = output_buf.t, output_buf.scales, output_buf.block_rows
     elems, n = (num_rows - 1) * apart + num_columns if num_rows > 0 else 0, -(-num_rows // m) * -(-num_columns // 128)
     # all of it in one expression: a call to _at for each tensor takes 0.2 us more
-    if not (x.dtype in _TYPES and x.numel() >= elems and x.is_contiguous()
+    if not (kind is not None and x.numel() >= elems and x.is_contiguous()
             and q.get_device() == here and q.dtype is _F8 and q.numel() >= num_rows * num_columns and q.is_contiguous()
             and scales.get_device() == here and scales.dtype is _F32 and scales.numel() >= n and scales.is_contiguous()):
         _at(name, x, elems, "input", _FLOATS, here)
         _at(name, q, num_rows * num_columns, "output", (_F8,), here)
         _at(name, scales, n, "scales", (_F32,), here)
-    check(lib().small_b200_quantize_blocks_f8(num_rows, num_columns, m, _TYPES[x.dtype], x.data_ptr(), apart, q.data_ptr(), scales.data_ptr(),
-                                              _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)))
+    rc = lib().small_b200_quantize_blocks_f8(num_rows, num_columns, m, kind, x.data_ptr(), apart, q.data_ptr(), scales.data_ptr(),
+                                             _stream_now(here) if stream is None else _stream(stream))
+    if rc:
+        check(rc)
 
 
 def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, out_stride, stream):
@@ -732,18 +744,20 @@ def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, o
         raise ValueError(f"{name}: Float8Buffer operands go together")
     if inp.block_rows != 1 or filt.block_rows != 128:
         raise ValueError(f"{name}: activations in blocks of 1 row and weights in blocks of 128, not {inp.block_rows} and {filt.block_rows}")
-    if (filt.rows, filt.columns) != (K, C_) or inp.columns != C_ or inp.rows < rows:
+    if filt.rows != K or filt.columns != C_ or inp.columns != C_ or inp.rows < rows:
         raise ValueError(f"{name}: weights {filt.rows} x {filt.columns} and activations {inp.rows} x {inp.columns} for {rows} rows, {C_} -> {K}")
-    y = _tensor(out)
-    if y.dtype not in _FLOATS:
+    y = out if isinstance(out, torch.Tensor) else out.t
+    kind = _TYPES.get(y.dtype)
+    if kind is None:
         raise ValueError(f"{name}: the output is a FloatBuffer, BFloat16Buffer or HalfBuffer")
-    _size(name, rows)
-    _size(name, K)
-    _size(name, C_)
-    apart = _stride(name, K, out_stride)
+    if not (0 <= rows < _MOST and 0 <= K < _MOST and 0 <= C_ < _MOST):
+        _sizes(name, rows, K, C_)
+    apart = K if out_stride is None else _stride(name, K, out_stride)
     # (a slope of -0.0 is another one than 0.0, but not another key)
-    L = (_dense_layer if slope or math.copysign(1.0, slope) > 0 else _dense_layer.__wrapped__)(rows, K, C_, _TYPES[y.dtype], apart, accumulate, act, slope)
-    blocks, here = -(-C_ // 128), _home(name, y, "output")
+    L = (_dense_layer if slope or math.copysign(1.0, slope) > 0 else _dense_layer.__wrapped__)(rows, K, C_, kind, apart, accumulate, act, slope)
+    blocks, here = -(-C_ // 128), y.get_device()
+    if here < 0 or here != _device_now():
+        _home(name, y, "output")
     elems = (rows - 1) * apart + K if rows > 0 else 0
     x, xs, w, ws = inp.t, inp.scales, filt.t, filt.scales
     if not (y.numel() >= elems and y.is_contiguous()
@@ -756,9 +770,11 @@ def _dense_f8(name, K, C_, inp, filt, bias, out, accumulate, act, slope, rows, o
         _at(name, xs, rows * blocks, "input scales", (_F32,), here)
         _at(name, w, K * C_, "filter", (_F8,), here)
         _at(name, ws, -(-K // 128) * blocks, "filter scales", (_F32,), here)
-    check(lib().small_b200_dense_f8(L, x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(),
-                                    None if bias is None else _at(name, _tensor(bias), K, "bias", (_F32,), here), y.data_ptr(),
-                                    _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)))
+    rc = lib().small_b200_dense_f8(L, x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(),
+                                   None if bias is None else _at(name, _tensor(bias), K, "bias", (_F32,), here), y.data_ptr(),
+                                   _stream_now(here) if stream is None else _stream(stream))
+    if rc:
+        check(rc)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -778,14 +794,15 @@ def LogProbabilities(num_rows, num_classes, logits_buf, tokens, logprobs_buf, en
     with logprobs_buf).  Classes at minus infinity are masked; a row with nothing else has log-probabilities of minus infinity and an entropy of 0.
     A row with NaN or plus infinity has NaN for both.  small::SoftMax (:1778 of the reference) subtracts no maximum and knows no classes."""
     name = "LogProbabilities"
-    _size(name, num_rows)
-    _size(name, num_classes)
-    _size(name, top)
-    apart = _stride(name, num_classes, row_stride)
-    x = _tensor(logits_buf)
-    here = _home(name, x, "logits")
+    if not (0 <= num_rows < _MOST and 0 <= num_classes < _MOST and 0 <= top < _MOST):
+        _sizes(name, num_rows, num_classes, top)
+    apart = num_classes if row_stride is None else _stride(name, num_classes, row_stride)
+    x = logits_buf if isinstance(logits_buf, torch.Tensor) else logits_buf.t
+    kind, here = _TYPES.get(x.dtype), x.get_device()
+    if here < 0 or here != _device_now():
+        _home(name, x, "logits")
     elems, each = (num_rows - 1) * apart + num_classes if num_rows > 0 else 0, num_rows * top
-    if not (x.dtype in _TYPES and x.numel() >= elems and x.is_contiguous()):
+    if not (kind is not None and x.numel() >= elems and x.is_contiguous()):
         _at(name, x, elems, "logits", _FLOATS, here)
     given = lp = h = tv = ti = None
     wide = 4
@@ -812,8 +829,10 @@ def LogProbabilities(num_rows, num_classes, logits_buf, tokens, logprobs_buf, en
         if not (top_tokens.get_device() == here and top_tokens.dtype is _I32 and top_tokens.numel() >= each and top_tokens.is_contiguous()):
             _at(name, top_tokens, each, "top tokens", (_I32,), here)
         ti = top_tokens.data_ptr()
-    check(lib().small_b200_logprobs(num_rows, num_classes, _TYPES[x.dtype], x.data_ptr(), apart, wide, given, lp, h, top, tv, ti,
-                                    _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)))
+    rc = lib().small_b200_logprobs(num_rows, num_classes, kind, x.data_ptr(), apart, wide, given, lp, h, top, tv, ti,
+                                   _stream_now(here) if stream is None else _stream(stream))
+    if rc:
+        check(rc)
 
 
 # --------------------------------------------------------------------------- detection head
