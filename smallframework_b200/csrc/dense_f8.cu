@@ -534,41 +534,39 @@ __device__ __forceinline__ void copy_bias(const DenseArgs &a, uint8_t *to, int k
     for (int c = 0; c < COLS; c += 32)
         copy4(to + (c + lane) * 4, a.bias + min(k0 + c + lane, a.K - 1));
 }
-// 128 bytes of each of a warp's 32 rows, from output k on, between the output and the warp's shared memory (OUT: to the output): element by element, a row at a
-// time on the way out, as many together on the way in as hide that a load takes its time.
+// 128 bytes of each of a warp's 32 rows, from output k on, between the output and the warp's shared memory (OUT: to the output): element by element, several rows
+// together, which hides that a load takes its time.
 template <int TYPE, bool OUT>
 __device__ __forceinline__ void by_element(const DenseArgs &a, uint8_t *stage, int first, int k)
 {
     using Word = typename std::conditional<TYPE == SMALL_B200_TYPE_F32, uint32_t, uint16_t>::type;
-    constexpr int VE = 16 / sizeof(Word), EACH = 8 * VE / 32, TOGETHER = OUT ? 1 : 8;
+    constexpr int VE = 16 / sizeof(Word), EACH = 8 * VE / 32, TOGETHER = OUT ? 4 : 8;
     const int lane = threadIdx.x & 31, rows = min(32, a.rows - first);
     Word *out = static_cast<Word *>(a.out) + (long long)first * a.out_stride + k;
 #pragma unroll 1
     for (int q0 = 0; q0 < rows; q0 += TOGETHER)
     {
-        Word old[TOGETHER][EACH];
-#pragma unroll
-        for (int n = 0; n < TOGETHER; ++n)
-#pragma unroll
-            for (int e = 0; e < EACH; ++e)
-            {
-                const int q = q0 + n, c = lane + 32 * e;
-                const bool has = q < rows && k + c < a.K;
-                Word *in = reinterpret_cast<Word *>(stage + q * 128 + ((c / VE ^ (q & 7)) << 4)) + c % VE;
-                if (OUT && has)
-                    out[q * a.out_stride + c] = *in;
-                else if (!OUT)
-                    old[n][e] = has ? out[q * a.out_stride + c] : (Word)0;
-            }
-        if (!OUT)
+        Word v[TOGETHER][EACH];
+        auto all = [&](auto each) {
 #pragma unroll
             for (int n = 0; n < TOGETHER; ++n)
 #pragma unroll
                 for (int e = 0; e < EACH; ++e)
                 {
                     const int q = q0 + n, c = lane + 32 * e;
-                    *(reinterpret_cast<Word *>(stage + q * 128 + ((c / VE ^ (q & 7)) << 4)) + c % VE) = old[n][e];
+                    each(v[n][e], reinterpret_cast<Word *>(stage + q * 128 + ((c / VE ^ (q & 7)) << 4)) + c % VE, out + q * a.out_stride + c, q < rows && k + c < a.K);
                 }
+        };
+        if (OUT)
+        {
+            all([](Word &v, Word *in, Word *, bool) { v = *in; });
+            all([](Word &v, Word *, Word *out, bool has) { if (has) *out = v; });
+        }
+        else
+        {
+            all([](Word &v, Word *, Word *out, bool has) { v = has ? *out : (Word)0; });
+            all([](Word &v, Word *in, Word *, bool) { *in = v; });
+        }
     }
 }
 
@@ -686,6 +684,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             uint8_t *stage = ring + MANY_STAGES * MANY_STAGE + (warp - 4) * STAGE_OUT;
             const int first = at.r0 + rank * 128 + (warp & 3) * 32; // row of the warp
             char *out = static_cast<char *>(a.out);
+            auto by_vector = [&](int c0) { return a.wide && (a.K % VE == 0 || k0 + c0 + WIDE <= a.K); }; // 16 bytes are this row's or behind its end
             if (FINISH && a.accumulate)
             {
                 // The old values, the same way in: whole lines of four rows, then every thread its row's.
@@ -694,14 +693,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                 {
                     if (k0 + c0 >= a.K)
                         break;
-                    if (a.wide && k0 + c0 + WIDE <= a.K)
+                    if (by_vector(c0))
                     {
                         uint4 old[8];
 #pragma unroll
                         for (int n = 0; n < 8; ++n)
                         {
                             const int q = n * 4 + (lane >> 3);
-                            if (first + q < a.rows)
+                            if (first + q < a.rows && k0 + c0 + (lane & 7) * VE < a.K)
                                 old[n] = *reinterpret_cast<const uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + (lane & 7) * VE) * SIZE);
                             else
                                 old[n] = make_uint4(0u, 0u, 0u, 0u);
@@ -787,13 +786,13 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                     *reinterpret_cast<uint4 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = w; // no two lanes of eight share banks
                 }
                 __syncwarp();
-                if (a.wide && k0 + c0 + WIDE <= a.K)
+                if (by_vector(c0))
                 {
 #pragma unroll
                     for (int n = 0; n < 8; ++n)
                     {
                         const int q = n * 4 + (lane >> 3), j = lane & 7;
-                        if (first + q < a.rows)
+                        if (first + q < a.rows && k0 + c0 + j * VE < a.K)
                             *reinterpret_cast<uint4 *>(out + ((long long)(first + q) * a.out_stride + k0 + c0 + j * VE) * SIZE) =
                                 *reinterpret_cast<const uint4 *>(stage + q * 128 + ((j ^ (q & 7)) << 4));
                     }
@@ -962,6 +961,19 @@ int launch_many(const DenseArgs &a, const CUtensorMap &map_x, const CUtensorMap 
     return launched(N == 256 ? "dense_f8_many_kernel<256>" : "dense_f8_many_kernel<128>");
 }
 
+// CTAs (a cluster) that share a reduction in the kernel for few rows.  Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each
+// at least two blocks.  Clusters of four and eight do not fill every group of SMs (148 SMs hold 70 and 33): 1 row, 4096 inputs, 70 tiles of outputs 9.0 us in fours and 9.9 in twos, but 72 tiles 13.4 and 10.0; 8192 inputs,
+// 33 tiles 8.0 in eights and 8.8 in fours, but 34 tiles 12.2 and 10.1.  Clusters of eight come up slowly (the last of 32 after 1.8 us, of 64 clusters of four
+// after 0.9), so short reductions are cut in eight only where four leave SMs without a CTA: 64 rows, 2048 inputs, 20 tiles 7.2 and 6.8, 15 tiles 5.5 and 6.5.
+int parts_of(long long tiles, int blocks)
+{
+    const long long sms = num_sms();
+    int parts = 1;
+    while (parts < 8 && blocks >= 4 * parts && tiles * 2 * parts <= (parts == 1 ? 2 * sms : parts == 2 ? 2 * sms - 16 : blocks >= 32 ? 2 * sms - 32 : sms))
+        parts *= 2;
+    return parts;
+}
+
 template <int TYPE>
 int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long in_stride, const void *filt, long long filt_stride, cudaStream_t st)
 {
@@ -969,30 +981,26 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
     if (!status)
         return fail(SMALL_B200_CUDA_ERROR, "device status word not available");
     CUtensorMap map_w, map_x;
-    // Microseconds that either kernel takes, fitted to 136 sizes of 64 to 512 rows, 64 to 8192 outputs and 512 to 8192 inputs (on average 0.2 % are lost against the
-    // faster one): a start and an end, a tile of 128 outputs by 64 rows and its blocks in the one, a wave of 256 x 256 tiles, or of halves of such tiles, in the
-    // other.  64 rows, 512 -> 4096: 5.6 us and 4.7; 128 rows, 4096 -> 4096: 10.9 and 12.9; 256 rows: 15.5 and 13.2; 512 rows, 8192 -> 1024: 15.1 and 21.9.
-    const double b = a.blocks, tiles_of_few = (double)((D->K + 127LL) / 128) * ((D->rows + 63LL) / 64);
+    // Microseconds that either kernel takes, fitted to 136 sizes of 64 to 512 rows, 64 to 8192 outputs and 512 to 8192 inputs (none of which loses 1 % against the
+    // faster one): a start and an end, a tile of 128 outputs by 64 rows and its blocks, a second CTA an SM in the one, a wave of 256 x 256 tiles, or of halves of
+    // such tiles, in the other.  64 rows, 512 -> 4096: 5.6 us and 4.7; 128 rows, 4096 -> 4096: 10.9 and 12.9; 256 rows: 15.5 and 13.2; 512 rows, 8192 -> 1024: 15.1 and 21.9.
+    const double b = a.blocks;
+    const long long tiles_of_few = ((D->K + 127LL) / 128) * ((D->rows + 63LL) / 64);
     const long long pairs_of_tiles = ((D->K + 255LL) / 256) * ((D->rows + 255LL) / 256), at_once = std::max(1, num_sms() / 2);
     // Tiles for which there are twice as many pairs of CTAs are done in halves, a launch of its own behind whole waves.
     const long long whole = pairs_of_tiles / at_once * at_once, rest = pairs_of_tiles - whole;
     const bool halves = rest > 0 && 2 * rest <= at_once;
-    const double few_us = 4.7 + 0.048 * b + tiles_of_few * (0.0095 + 0.00203 * b), wave = 0.47 * b + 1.9;
-    const double many_us = 3.2 + (double)(whole / at_once) * wave + (rest == 0 ? 0. : halves ? 0.285 * b + (whole > 0 ? 3.2 : 0.) : wave);
+    const double few_us = 5.06 + 0.022 * b + (double)tiles_of_few * (0.0062 + 0.0023 * b) + (tiles_of_few * parts_of(tiles_of_few, a.blocks) > num_sms() ? 0.37 : 0.);
+    const double wave = 0.47 * b + 1.9;
+    // (its way out takes longer in fp32 and behind a bias or an activation, once a launch; the other's hardly does)
+    const double many_us = 3.2 + (double)(whole / at_once) * wave + (rest == 0 ? 0. : halves ? 0.285 * b + (whole > 0 ? 3.2 : 0.) : wave) +
+                           (TYPE == SMALL_B200_TYPE_F32 ? 0.7 : 0.) + (D->act != SMALL_B200_ACT_NONE || a.bias ? 0.5 : 0.);
     if (D->rows <= 32 || few_us < many_us)
     {
         const int bn = D->rows <= 16 ? 16 : D->rows <= 32 ? 32 : 64;
         a.k_tiles = (D->K + 127) / 128;
         a.r_tiles = (D->rows + bn - 1) / bn;
-        // Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each at least two blocks.  Clusters of four and eight do not fill every
-        // group of SMs (148 SMs hold 70 and 33): 1 row, 4096 inputs, 70 tiles of outputs 9.0 us in fours and 9.9 in twos, but 72 tiles 13.4 and 10.0; 8192 inputs,
-        // 33 tiles 8.0 in eights and 8.8 in fours, but 34 tiles 12.2 and 10.1.  Clusters of eight come up slowly (the last of 32 after 1.8 us, of 64 clusters of four
-        // after 0.9), so short reductions are cut in eight only where four leave SMs without a CTA: 64 rows, 2048 inputs, 20 tiles 7.2 and 6.8, 15 tiles 5.5 and 6.5.
-        const long long tiles = (long long)a.k_tiles * a.r_tiles, sms = num_sms();
-        a.split = 1;
-        while (a.split < 8 && a.blocks >= 4 * a.split &&
-               tiles * 2 * a.split <= (a.split == 1 ? 2 * sms : a.split == 2 ? 2 * sms - 16 : a.blocks >= 32 ? 2 * sms - 32 : sms))
-            a.split *= 2;
+        a.split = parts_of((long long)a.k_tiles * a.r_tiles, a.blocks);
         if (int rc = map_rows(&map_w, filt, D->K, D->C, filt_stride, 128))
             return rc;
         if (int rc = map_rows(&map_x, in, D->rows, D->C, in_stride, bn))
