@@ -78,28 +78,5 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-// Eight consecutive elements from element `at`, zeros where `has` is false; VEC: `at` is on a 16-byte boundary.
-template <int TYPE, bool VEC>
-__device__ __forceinline__ void load8(const void *p, long long at, bool has, float *x)
-{
-    if (!VEC)
-    {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[i] = has ? load1<TYPE>(p, at + i) : 0.f;
-    }
-    else if (TYPE == SMALL_B200_TYPE_F32)
-    {
-        const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at);
-        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = has ? __ldg(q) : z, b = has ? __ldg(q + 1) : z;
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    }
-    else
-    {
-        const uint4 w = has ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at)) : make_uint4(0u, 0u, 0u, 0u);
-        unpack2<TYPE>(w.x, x[0], x[1]); unpack2<TYPE>(w.y, x[2], x[3]); unpack2<TYPE>(w.z, x[4], x[5]); unpack2<TYPE>(w.w, x[6], x[7]);
-    }
-}
 #endif
 } // namespace sb

@@ -8,7 +8,7 @@
 // Bound: memory (2 or 4 bytes read and one written an element), and close behind it the integer ALU (70 % of its slots at 8192x8192 bf16: unpacking, conversions,
 // packing).  16 lanes own 8 columns each of a block, so the largest magnitude of a row block is four shuffles away and nothing is read twice; four blocks a
 // lane are under way, and 16-bit values are compared two at a time as they are.
-// Measured on a B200: 8192x8192 bf16 40.5 us (5.0 TB/s, 31.2 at the copy rate), 5000x4112 fp32 in square blocks 20.7 us (5.0 TB/s, 15.9), 1x4096 2.0 us.
+// Measured on a B200: 8192x8192 bf16 40.5 us (5.0 TB/s, 31.2 at the copy rate), 5000x4112 fp32 in square blocks 19.2 us (5.4 TB/s, 15.9), 1x4096 2.0 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -166,6 +166,27 @@ struct Raw8
                 w[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
     }
+    // Infinities take no part in a scale and become NaN, as NaN does.
+    __device__ __forceinline__ void infinities_to_nan()
+    {
+        constexpr int N = TYPE == SMALL_B200_TYPE_F32 ? 2 : 1;
+        constexpr uint32_t INF = TYPE == SMALL_B200_TYPE_F32 ? 0x7f800000u : TYPE == SMALL_B200_TYPE_BF16 ? 0x7f80u : 0x7c00u;
+        constexpr uint32_t QUIET = TYPE == SMALL_B200_TYPE_F32 ? 0x400000u : TYPE == SMALL_B200_TYPE_BF16 ? 0x40u : 0x200u;
+        auto word = [](uint32_t &v) {
+            if (TYPE == SMALL_B200_TYPE_F32)
+                v |= (v & 0x7fffffffu) == INF ? QUIET : 0u;
+            else
+                v |= ((v & 0x7fffu) == INF ? QUIET : 0u) | ((v >> 16 & 0x7fffu) == INF ? QUIET << 16 : 0u);
+        };
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            word(w[i].x);
+            word(w[i].y);
+            word(w[i].z);
+            word(w[i].w);
+        }
+    }
     __device__ __forceinline__ void unpack(float *x) const
     {
         if (TYPE == SMALL_B200_TYPE_F32)
@@ -180,6 +201,23 @@ struct Raw8
         }
     }
 };
+// Of 16-bit values, two at a time, as they are: the larger ones, and the largest magnitudes of eight.
+template <int TYPE>
+__device__ __forceinline__ uint32_t max_of_pairs(uint32_t a, uint32_t b)
+{
+    uint32_t c;
+    if (TYPE == SMALL_B200_TYPE_BF16)
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    else
+        asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    return c;
+}
+template <int TYPE>
+__device__ __forceinline__ uint32_t magnitudes(const Raw8<TYPE> &r)
+{
+    constexpr uint32_t MAG = 0x7fff7fffu;
+    return max_of_pairs<TYPE>(max_of_pairs<TYPE>(r.w[0].x & MAG, r.w[0].y & MAG), max_of_pairs<TYPE>(r.w[0].z & MAG, r.w[0].w & MAG));
+}
 // The largest magnitude of the 16 lanes' values; a NaN is not seen.
 template <int TYPE>
 __device__ __forceinline__ float block_max(const Raw8<TYPE> &r, const float *x)
@@ -192,20 +230,10 @@ __device__ __forceinline__ float block_max(const Raw8<TYPE> &r, const float *x)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         return m;
     }
-    // two at a time, as they are
-    auto max2 = [](uint32_t a, uint32_t b) {
-        uint32_t c;
-        if (TYPE == SMALL_B200_TYPE_BF16)
-            asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
-        else
-            asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
-        return c;
-    };
-    constexpr uint32_t MAG = 0x7fff7fffu;
-    uint32_t m = max2(max2(r.w[0].x & MAG, r.w[0].y & MAG), max2(r.w[0].z & MAG, r.w[0].w & MAG));
+    uint32_t m = magnitudes<TYPE>(r);
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1)
-        m = max2(m, __shfl_xor_sync(0xffffffffu, m, d));
+        m = max_of_pairs<TYPE>(m, __shfl_xor_sync(0xffffffffu, m, d));
     float lo, hi;
     unpack2<TYPE>(m, lo, hi);
     return fmaxf(fmaxf(lo, hi), 0.f); // 0 where all are NaN
@@ -276,31 +304,48 @@ __global__ void __launch_bounds__(ROW_THREADS, TYPE == SMALL_B200_TYPE_F32 ? 4 :
         finish_block<TYPE>(r[j], has[j], out + to[j], scales + u0 + j * GROUPS, lane);
 }
 
-// A CTA owns a square block: 16 lanes by 16 rows at a time, eight times, all of it in registers.
+// A CTA owns a square block: 16 lanes by 16 rows at a time, eight times, all of it in registers, 16-bit values as they are.  A block's loads and stores take turns,
+// so it is CTAs that hide them: 5000x4112 fp32 20.9 us with two an SM, 19.2 with three; 8192x8192 bf16 56 with two (values kept as floats), 45 with three, 41.5 with four.
 template <int TYPE, bool VEC>
-__global__ void __launch_bounds__(256) quantize_square_f8_kernel(const QuantArgs a, const void *__restrict__ in, uint8_t *__restrict__ out,
-                                                                   float *__restrict__ scales)
+__global__ void __launch_bounds__(256, TYPE == SMALL_B200_TYPE_F32 ? 3 : 4)
+    quantize_square_f8_kernel(const QuantArgs a, const void *__restrict__ in, uint8_t *__restrict__ out, float *__restrict__ scales)
 {
     __shared__ float part[8];
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
     const int br = a.by_blocks.div((int)blockIdx.x), bc = (int)blockIdx.x - br * a.blocks;
     const int c = bc * 128 + lane * 8;
-    float x[8][8];
+    Raw8<TYPE> r[8];
     previous_kernel_done();
     next_kernel_may_start();
 #pragma unroll
     for (int j = 0; j < 8; ++j)
     {
         const int row = br * 128 + j * 16 + group;
-        const bool has = row < a.rows && c < a.columns;
-        load8<TYPE, VEC>(in, (long long)row * a.stride + c, has, x[j]);
+        r[j].template load<VEC>(in, (long long)row * a.stride + c, row < a.rows && c < a.columns);
     }
     for (int pass = 0;; ++pass)
     {
         float m = 0.f;
+        if (TYPE == SMALL_B200_TYPE_F32)
+        {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            m = fmaxf(m, abs_max8(x[j]));
+            for (int j = 0; j < 8; ++j)
+            {
+                float x[8];
+                r[j].unpack(x);
+                m = fmaxf(m, abs_max8(x));
+            }
+        }
+        else
+        {
+            uint32_t most = magnitudes<TYPE>(r[0]);
+#pragma unroll
+            for (int j = 1; j < 8; ++j)
+                most = max_of_pairs<TYPE>(most, magnitudes<TYPE>(r[j]));
+            float lo, hi;
+            unpack2<TYPE>(most, lo, hi);
+            m = fmaxf(fmaxf(lo, hi), 0.f); // 0 where all are NaN
+        }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
@@ -315,7 +360,7 @@ __global__ void __launch_bounds__(256) quantize_square_f8_kernel(const QuantArgs
         {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                infinities_to_nan(x[j]);
+                r[j].infinities_to_nan();
             __syncthreads();
             continue;
         }
@@ -325,7 +370,11 @@ __global__ void __launch_bounds__(256) quantize_square_f8_kernel(const QuantArgs
         {
             const int row = br * 128 + j * 16 + group;
             if (row < a.rows && c < a.columns)
-                *reinterpret_cast<uint2 *>(out + (long long)row * a.columns + c) = quantize8(x[j], scale, inv);
+            {
+                float x[8];
+                r[j].unpack(x);
+                *reinterpret_cast<uint2 *>(out + (long long)row * a.columns + c) = quantize8(x, scale, inv);
+            }
         }
         if (threadIdx.x == 0)
             scales[blockIdx.x] = scale;
@@ -338,7 +387,7 @@ int launch_quantize(const QuantArgs &a, int block_rows, const void *in, uint8_t 
 {
     if (block_rows == 128)
     {
-        const Launch l((unsigned)a.units, 256, 0, st, 0, a.units <= 2 * num_sms());
+        const Launch l((unsigned)a.units, 256, 0, st, 0, a.units <= 3LL * num_sms());
         SB_CUDA(cudaLaunchKernelEx(&l.cfg, quantize_square_f8_kernel<TYPE, VEC>, a, in, out, scales));
         return launched("quantize_square_f8_kernel");
     }
