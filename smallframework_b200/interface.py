@@ -121,7 +121,10 @@ class HalfBuffer(_NarrowBuffer):
 
 class Float8Buffer(_NarrowBuffer):
     """A matrix [rows][columns] of e4m3 codes (in `t`) with an fp32 scale (in `scales`) for each block of 128 columns by `block_rows` rows:
-    1 for activations, 128 for weights.  The value of an element is its code times its block's scale."""
+    1 for activations, 128 for weights.  The value of an element is its code times its block's scale.
+
+    data: codes, as float8_e4m3fn or as bytes (uint8), in torch or numpy; numbers of other types are refused, QuantizeBlocks takes those.
+    scales: fp32, by blocks; 1 where only data is given."""
     dtype = torch.float8_e4m3fn
 
     def __init__(self, rows, columns, block_rows=1, device="cuda", data=None, scales=None):
@@ -129,12 +132,24 @@ class Float8Buffer(_NarrowBuffer):
             raise ValueError(f"Float8Buffer: blocks of 1 or 128 rows, not {block_rows}")
         self.rows, self.columns, self.block_rows = int(rows), int(columns), block_rows
         n = -(-self.rows // block_rows) * -(-self.columns // 128)
-        if isinstance(data, np.ndarray):  # codes
-            data = torch.from_numpy(np.ascontiguousarray(data, np.uint8)).view(self.dtype)
+        if data is not None:
+            data = self._codes(data)
         super().__init__(self.rows * self.columns, device, data)
-        self.scales = torch.empty(n, device=device) if scales is None else _to_device(scales, torch.float32, device)
+        if scales is None:  # written by QuantizeBlocks, or those of plain codes
+            self.scales = torch.empty(n, device=device) if data is None else torch.ones(n, device=device)
+        else:
+            self.scales = _to_device(scales, torch.float32, device)
         if self.t.numel() != self.rows * self.columns or self.scales.numel() != n:
             raise ValueError(f"Float8Buffer: {self.t.numel()} codes and {self.scales.numel()} scales for {self.rows} x {self.columns}")
+
+    @classmethod
+    def _codes(cls, data):
+        """Bytes as the codes that they are.  (A conversion would take them for numbers, and numbers for bytes.)"""
+        if isinstance(data, np.ndarray) and data.dtype == np.uint8:
+            data = torch.from_numpy(np.ascontiguousarray(data))
+        if isinstance(data, torch.Tensor) and data.dtype in (torch.uint8, cls.dtype):
+            return data.contiguous().view(cls.dtype)
+        raise ValueError(f"Float8Buffer: codes are bytes or {cls.dtype}, not {getattr(data, 'dtype', type(data).__name__)}; QuantizeBlocks makes them from numbers")
 
     def dequantized(self):
         """The values as an fp32 tensor [rows][columns]."""
