@@ -124,7 +124,7 @@ __device__ __forceinline__ float4 bias4(const DenseArgs &a, int k)
     if (a.bias)
     {
         const int last = a.K - 1;
-        b = make_float4(__ldg(a.bias + min(k, last)), __ldg(a.bias + min(k + 1, last)), __ldg(a.bias + min(k + 2, last)), __ldg(a.bias + min(k + 3, last)));
+        b = make_float4(a.bias[min(k, last)], a.bias[min(k + 1, last)], a.bias[min(k + 2, last)], a.bias[min(k + 3, last)]);
     }
     return b;
 }
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
     auto ask = [&](int c) {
 #pragma unroll
         for (int j = 0; j < G::CHUNK; ++j)
-            sw[j] = c * G::CHUNK + j < n ? __ldg(a.filt_scales + (size_t)kt * a.blocks + b0 + c * G::CHUNK + j) : 0.f;
+            sw[j] = c * G::CHUNK + j < n ? a.filt_scales[(size_t)kt * a.blocks + b0 + c * G::CHUNK + j] : 0.f;
 #pragma unroll
         for (int q = 0; q < ROWS; ++q)
         {
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
             for (int j = 0; j < G::CHUNK; ++j)
             {
                 const int b = c * G::CHUNK + j;
-                sv[q][j] = col < BN && row < a.rows && b < n ? __ldg(sx + b) : 0.f;
+                sv[q][j] = col < BN && row < a.rows && b < n ? sx[b] : 0.f;
             }
         }
     };
@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
             // barrier is asked one step before its answer is needed.
             if (FINISH && a.bias && !a.accumulate) // asked for now, needed at the end, and until then not in registers
                 copy_bias<COLS>(a, ring + MANY_STAGES * MANY_STAGE + (warp - 4) * STAGE_OUT, k0);
-            float next_x = __ldg(sx), next_w = __ldg(sw); // multiplied when they are needed: until then nothing waits for them
+            float next_x = sx[0], next_w = sw[0]; // multiplied when they are needed: until then nothing waits for them
             uint32_t r[2][32];
             ok = __all_sync(0xffffffffu, mbar_wait(&sum_full[i % BUFS], (i / BUFS) & 1, status, 111));
             if (!ok)
@@ -646,8 +646,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) dense_f8_many_kernel(const __
                 const bool more = b + 1 < a.blocks;
                 if (more)
                 {
-                    next_x = __ldg(sx + b + 1);
-                    next_w = __ldg(sw + b + 1);
+                    next_x = sx[b + 1];
+                    next_w = sw[b + 1];
                 }
                 bool ready = false;
 #pragma unroll

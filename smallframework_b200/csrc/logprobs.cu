@@ -118,7 +118,7 @@ __device__ __forceinline__ uint4 load_vector(const void *row, int v, int skew, i
     constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8;
     const long long first = (long long)v * VE - skew;
     if (first >= 0 && first + VE <= classes)
-        return __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(row) + first * (16 / VE)));
+        return *reinterpret_cast<const uint4 *>(static_cast<const char *>(row) + first * (16 / VE));
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -292,8 +292,7 @@ struct Shared
 
 template <int TYPE, int WARPS>
 __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_F32 ? 4 : 5)
-    logprobs_kernel(const LogpArgs a, const void *__restrict__ logits, const void *__restrict__ tokens, float *__restrict__ logprobs,
-                    float *__restrict__ entropy, float *__restrict__ top_logprobs, int *__restrict__ top_tokens, int *status)
+    logprobs_kernel(const LogpArgs a, const void *logits, const void *tokens, float *logprobs, float *entropy, float *top_logprobs, int *top_tokens, int *status)
 {
     constexpr int VE = TYPE == SMALL_B200_TYPE_F32 ? 4 : 8, SIZE = 16 / VE, BATCH = 4, THREADS = 32 * WARPS;
     constexpr int ROOM = sizeof(Shared<WARPS>::found) / 8;
@@ -399,7 +398,7 @@ __global__ void __launch_bounds__(256, WARPS == 1 ? 3 : TYPE == SMALL_B200_TYPE_
             float vm[BATCH];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j)
-                w[j] = j == 0 && v < whole0 ? load_vector<TYPE>(row, v, skew, a.classes) : __ldg(aligned + v + j * THREADS);
+                w[j] = j == 0 && v < whole0 ? load_vector<TYPE>(row, v, skew, a.classes) : aligned[v + j * THREADS];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j)
                 vm[j] = vector_max<TYPE>(w[j]);

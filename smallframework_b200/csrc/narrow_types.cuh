@@ -39,6 +39,8 @@ struct Launch
 };
 
 #ifdef __CUDACC__
+// What the kernel before wrote is read by plain loads behind the wait: __ldg and const __restrict__ are for data that nobody writes while a kernel exists, and
+// the compiler may move such loads over the wait.
 __device__ __forceinline__ void previous_kernel_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // The two 16-bit floats of a word.
