@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(FEW_THREADS) dense_f8_few_kernel(const __grid_
         }
         __syncwarp();
         asm volatile("bar.arrive 1, %0;" ::"n"(FEW_THREADS) : "memory");
-        if (!a.behind) // what this launch reads the launch before it has waited for, before it let this one start
+        if (!a.behind) // the other launch of the call has waited for what both read, before it let this one start, and writes nothing that this one reads
             previous_kernel_done();
         next_kernel_may_start();
         if (elect_one())
@@ -940,6 +940,7 @@ int launch_few(const DenseArgs &a, const CUtensorMap &map_w, const CUtensorMap &
         SB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
         configured.mark(dev);
     }
+    // early for any number of waves: its CTAs are few and long
     const Launch l((unsigned)(a.count * a.split), FEW_THREADS, G::SMEM, st, a.split > 1 ? (unsigned)a.split : 0u);
     SB_CUDA(cudaLaunchKernelEx(&l.cfg, kern, map_w, map_x, a, status));
     return launched("dense_f8_few_kernel");

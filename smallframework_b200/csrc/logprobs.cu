@@ -717,7 +717,9 @@ int launch_logprobs(const LogpArgs &a, const void *logits, const void *tokens, f
     int *status = device_status_ptr();
     if (!status)
         return fail(SMALL_B200_CUDA_ERROR, "device status word not available");
-    const Launch l((unsigned)(WARPS == 1 ? (a.rows + 7) / 8 : a.rows * a.split), 256, 0, st, a.split > 1 ? (unsigned)a.split : 0u, a.rows * a.split <= 4LL * num_sms());
+    const long long grid = WARPS == 1 ? (a.rows + 7) / 8 : a.rows * a.split;
+    // early where all CTAs are resident at once, three an SM or four (fp32; 3500 rows of 2000 a call of its own each 10.0 us, 12.3 otherwise)
+    const Launch l((unsigned)grid, 256, 0, st, a.split > 1 ? (unsigned)a.split : 0u, grid <= (WARPS == 1 ? 3LL : 4LL) * num_sms());
     SB_CUDA(cudaLaunchKernelEx(&l.cfg, logprobs_kernel<TYPE, WARPS>, a, logits, tokens, logprobs, entropy, top_logprobs, (int *)top_tokens, status));
     return launched("logprobs_kernel");
 }

@@ -17,8 +17,10 @@ inline int type_size(int type)
 // A launch of clusters of `cluster` CTAs along x, 0 for none (the kernels then use no cluster instructions: stores to shared::cluster and cluster barriers raised
 // illegal instructions in a launch without clusters).  With `early` it may come up while the kernel before it in its stream ends: its kernel sets itself up,
 // calls previous_kernel_done() before it touches global memory, and next_kernel_may_start() once; what comes behind it waits for the whole of it all the same.
+// (One launch reads without that wait: the second of a dense layer on few rows that is two launches, whose first one has waited.)
 // Calls in a row on a B200: dense 1 row, 2048 -> 512, 4.3 us and 3.2, 4096 -> 4096 5.8 and 5.4; but the quantisation of 8192x8192, whose 8192 CTAs come and
-// go, 40.5 and 46.2: early only where the grid is resident at once.
+// go, 40.5 and 46.2: early only where the grid is resident at once, or is a few waves of long CTAs (dense on few rows, up to four waves: 1 row, 512 -> 40000, 12.2 us
+// and 9.9, 1024 -> 131072 32.6 and 30.0; 64 rows, 1920 -> 60000, 33.9 and 31.7).
 struct Launch
 {
     cudaLaunchConfig_t cfg = {};

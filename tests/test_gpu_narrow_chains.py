@@ -63,3 +63,33 @@ def test_old_outputs_read_by_the_next_call(kind, rows, K, C_):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [8, 600, 3000, 3552, 3553, 9000])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rows_of_a_warp_each_behind_what_writes_them(rows, kind):
+    """Log-probabilities that start early (grids that are resident at once) and that do not, behind a dense layer and before one that writes the logits anew."""
+    K, C_ = 701, 128
+    w, xs = U.operand(K, C_, 128, 1, spread_of_scales=0.0), [U.operand(rows, C_, 1, s, spread_of_scales=0.0) for s in (2, 3, 4)]
+    y, tokens = torch.zeros(rows * K, device="cuda", dtype=U.TYPES[kind]), torch.arange(rows, device="cuda") % K
+    out = [(torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda"), torch.zeros(rows * 3, device="cuda"), torch.zeros(rows * 3, dtype=torch.int32, device="cuda"))
+           for _ in range(6)]
+
+    def run(wait):
+        for n, (lp, h, tv, ti) in enumerate(out):
+            S.Dense(K, C_, xs[n % 3], w, U.buffer(y), batch=rows)
+            wait()
+            S.LogProbabilities(rows, K, U.buffer(y), tokens, U.buffer(lp), U.buffer(h), U.buffer(tv), ti, top=3)
+            wait()
+
+    run(torch.cuda.synchronize)
+    want = [[t.clone() for t in o] for o in out]
+    assert not torch.equal(want[0][0], want[1][0])
+    for _ in range(5):
+        for o in out:
+            for t in o:
+                t.zero_()
+        run(lambda: None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for o, v in zip(out, want) for a, b in zip(o, v))
+    assert _lib.device_status() == 0
