@@ -111,8 +111,9 @@ __device__ __forceinline__ void infinities_to_nan(float *x)
     for (int i = 0; i < 8; ++i)
         x[i] = fabsf(x[i]) == INFINITY ? NAN : x[i];
 }
-// amax / 448, rounded to nearest: the product with the rounded inverse and one correction by its exact remainder give every quotient from 2^-126 on
-// (all 2^23 significands of a dozen exponents were compared), in a sixth of a division's instructions.
+// amax / 448, rounded to nearest: the product with the rounded inverse and one correction by its exact remainder (P. Markstein, "Computation of elementary functions
+// on the IBM RISC System/6000 processor", 1990) give every quotient from 2^-126 on, in a sixth of a division's instructions; a test compares all significands of exponents
+// over the whole range.
 __device__ __forceinline__ float scale_of(float amax)
 {
     constexpr float INV = 1.f / F8_MAX;
