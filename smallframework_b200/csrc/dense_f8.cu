@@ -8,11 +8,12 @@
 // Two kernels:
 //   few    weights are the 128 lanes, 16, 32 or 64 rows of activations the columns.  The weights' bytes bound it: they come once, by TMA, into all SMs,
 //          the reduction cut among the CTAs of a cluster where output tiles are few; the parts go to the CTA that finishes them by asynchronous stores and are
-//          added in order.  On a B200: 1 row, 4096 -> 4096 5.4 us (2.6 at the copy rate), 24 rows, 8192 -> 8192 15.3 (10.5): a microsecond until the first sums, one
-//          and a half for the exchange and the end, the launch; in between the weights come at 6.0 TB/s.
+//          added in order.  On a B200, cold: 1 row, 4096 -> 4096 6.4 us (2.6 at the copy rate; 5.0 with the weights in L2), 24 rows, 8192 -> 8192 15.1 (10.5): a
+//          microsecond until the first sums, one and a half for the exchange and the end, the launch; in between the weights come at 6.0 TB/s.
 //   many   256 rows of activations by 256 outputs for a pair of CTAs.  A block takes 975 cycles where its MMAs take 512: 32 KB an SM come from L2 at the device's
 //          10.4 TB/s in 840, and tensor memory holds two blocks' sums, whose way to the registers and back is 1400 cycles for the two.  From 4096 rows on the
-//          1 kW power cap (1.46 GHz) comes first.  2048 rows, 4096 -> 8192 69 us (1.99 PFLOP/s), with bias and ReLU 71, onto old fp16 values 79; 8192, 8192 -> 8192 502 to 570 us.
+//          1 kW power cap comes first.  2048 rows, 4096 -> 8192 69 us (2.0 PFLOP/s), with bias and ReLU 71, onto old fp16 values 80; in runs of a second (1.58 GHz) 79, 82 and 90.
+//          8192 rows, 8192 -> 8192 481 us, in runs of a second (1.44 GHz) 555.
 #include <algorithm>
 #include <type_traits>
 
@@ -504,6 +505,7 @@ static_assert(MANY_STAGES % 2 == 0, "a buffer's blocks keep to every other stage
 constexpr int STAGE_OUT = 32 * 128; // a warp's way out
 constexpr int MANY_SMEM = 1024 + MANY_STAGES * MANY_STAGE + MANY_EPI * STAGE_OUT;
 // Registers: 384 threads start with 168 each (64512 in all); the four warps that feed keep 40, the eight that fold take 232, which adds up to the same.
+// (ptxas sees 168 for all of them: with a bias, an activation or old values 20 to 28 bytes a thread are spilled; so are 24 in the kernel for few rows with 32 and 64 columns.)
 constexpr int REGS_FEED = 40, REGS_FOLD = 232;
 constexpr int GROUP = 8; // tiles of rows that are walked together: their activations and the weights beside them stay in L2
 
@@ -967,8 +969,8 @@ int launch_many(const DenseArgs &a, const CUtensorMap &map_x, const CUtensorMap 
     return launched(N == 256 ? "dense_f8_many_kernel<256>" : "dense_f8_many_kernel<128>");
 }
 
-// CTAs (a cluster) that share a reduction in the kernel for few rows.  Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and leaves each
-// at least two blocks.  Clusters of four and eight do not fill every group of SMs (148 SMs hold 70 and 33): 1 row, 4096 inputs, 70 tiles of outputs 9.0 us in fours and 9.9 in twos, but 72 tiles 13.4 and 10.0; 8192 inputs,
+// CTAs (a cluster) that share a reduction in the kernel for few rows.  Two CTAs an SM fit; a reduction is cut while that adds CTAs to a first wave and there are
+// two blocks to a CTA.  The first CTAs take the rounded-up share and the last ones what is left, which may be nothing: 17 blocks in eight parts are 3, 3, 3, 3, 3, 2, 0 and 0.  Clusters of four and eight do not fill every group of SMs (148 SMs hold 70 and 33): 1 row, 4096 inputs, 70 tiles of outputs 9.0 us in fours and 9.9 in twos, but 72 tiles 13.4 and 10.0; 8192 inputs,
 // 33 tiles 8.0 in eights and 8.8 in fours, but 34 tiles 12.2 and 10.1.  Clusters of eight come up slowly (the last of 32 after 1.8 us, of 64 clusters of four
 // after 0.9), so short reductions are cut in eight only where four leave SMs without a CTA: 64 rows, 2048 inputs, 20 tiles 7.2 and 6.8, 15 tiles 5.5 and 6.5.
 int parts_of(long long tiles, int blocks)
@@ -1019,7 +1021,7 @@ int dispatch(const small_b200_dense *D, DenseArgs a, const void *in, long long i
                                                                                         : launch_few<64, TYPE>(a, map_w, map_x, status, st);
         };
         // A last wave that is not full is a launch of its own with the reductions cut, beside the end of the one before.  One launch and two: 1 row, 4096 -> 50257
-        // 42.5 us and 39.8, 64 rows 55.0 and 48.4; 24 rows, 2048 -> 39680 24.8 and 21.9; but 1024 -> 50257 17.2 and 17.6, 512 -> 50257 10.6 and 11.5.
+        // 39.5 us and 36.8, 64 rows 53.0 and 46.1; 24 rows, 2048 -> 39680 24.7 and 21.5; but (in an earlier build) 1024 -> 50257 17.2 and 17.6, 512 -> 50257 10.6 and 11.5.
         const int tiles = a.k_tiles * a.r_tiles, resident = 2 * num_sms(), full = tiles / resident * resident;
         if (full > 0 && tiles > full && a.blocks >= 16 && parts_of(tiles - full, a.blocks) > 1)
         {

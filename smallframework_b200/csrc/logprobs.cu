@@ -13,8 +13,9 @@
 // Bound: memory, every logit read once, then the special-function pipe (62 % of its slots: an exponential a logit).  A row is cut among the CTAs of a cluster where
 // rows are few, and what they found is merged over distributed shared memory (asynchronous stores to the first CTA): no workspace, and sums are always added in
 // the same order.  Short rows, and longer ones where there are many, go to a warp each, which needs no barrier.
-// Measured on a B200: 2048x131072 bf16 with 8 alternatives 101 to 105 us (5.1 TB/s; 92 without alternatives; 83 at the copy rate), 6x131072 fp32 with 20
-// alternatives 10.0 us (11.0 where rows are masked), 160x50257 fp16 with 10 12.2, 4096x1000 fp32 with 8 12.9 us, 1x1000 with 5 5.1 us.
+// Measured on a B200, cold: 2048x131072 bf16 with 8 alternatives 101 us (5.3 TB/s; 92 without alternatives; 83 at the copy rate; in runs of a second, at 1.73 GHz, 109 and
+// 102), 6x131072 fp32 with 20 alternatives 9.6 us (10.3 where rows are masked), 160x50257 fp16 with 10 14.1 (14.6; in L2 11.2 and 12.3), 4096x1000 fp32 with 8 15.3 us (in L2
+// 12.7), 1x1000 with 5 4.8 us.
 #include <algorithm>
 
 #include "narrow_types.cuh"
@@ -753,9 +754,9 @@ extern "C" int small_b200_logprobs(int32_t rows, int32_t classes, int32_t in_typ
     LogpArgs a;
     a.rows = rows; a.stride = stride ? stride : classes; a.classes = classes; a.top = top; a.token_bytes = token_bytes;
     // CTAs to a row, while each of their threads has a vector of its own.  What a CTA does besides reading (the best alternatives, the cluster) is 4 to 5 us, so more
-    // of them than two an SM pay only for rows of 256 KB on, and eight a row only for few of such rows.  With 8 alternatives, one, two and four CTAs a row:
-    // 160 rows of 131072 fp32 classes 34.3, 25.4 and 30.4 us, of 50257 fp16 11.1, 11.2, 13.7; 148 rows of 50257 9.9, 9.7, 12.4; 592 of 131072 fp32 52.5, 60.6, 78.3.
-    // Four and eight: 6 rows of 131072 fp32 9.8 and 8.6, of 50257 fp16 8.3 and 8.8.
+    // of them than two an SM pay only for rows of 256 KB on, and eight a row only for few of such rows.  With 8 alternatives, cold, one, two and four CTAs a row:
+    // 160 rows of 131073 fp32 classes 33.7, 25.0 and 30.7 us, of 50259 fp16 13.9, 12.9 and 14.0 (50257 in L2 11.1, 11.2, 13.7); 148 rows of 50259 13.3, 12.2 and 13.6; 592 of
+    // 131073 fp32 53.4, 61.1 and 78.9.  Four and eight: 6 rows of 131073 fp32 10.3 and 9.1, of 50259 fp16 8.0 and 8.7.
     const bool longer = (long long)classes * size >= 256 << 10;
     a.split = 1;
     while (a.split < (longer ? MAX_SPLIT : MAX_SPLIT / 2) && rows * 2LL * a.split <= (a.split == 1 && longer ? 4LL : a.split < 4 ? 2LL : 1LL) * num_sms() &&
@@ -764,9 +765,10 @@ extern "C" int small_b200_logprobs(int32_t rows, int32_t classes, int32_t in_typ
     if ((long long)rows * a.split > 0x7fffffffLL)
         return fail(SMALL_B200_INVALID_ARGUMENT, std::string(name) + " ERROR: too many rows.");
     cudaStream_t st = as_stream(stream);
-    // A warp to a row or a CTA to a row, without and with 8 alternatives: 1 row of 500 fp32 classes 3.1/5.0 us and 2.8/5.8, of 1000 3.5/5.4 and 2.9/4.9; 300 rows of
-    // 700 3.5/5.4 and 4.0/10.2, of 2000 5.3/7.2 and 4.6/7.1; where the warps of all rows fill the SMs 1000 rows of 4000 7.6/10.0 and 10.4/14.7, of 8000 10.6/13.3 and
-    // 11.9/16.3, of 16000 28.1/32.0 and 18.9/23.5; 4096 rows of 4000 24/29 and 41/56; in bf16 1000 rows of 16000 12.7/16.7 and 12.7/18.2, of 32000 31.7/37.5 and 20.4/25.7.
+    // A warp to a row or a CTA to a row, without and with 8 alternatives, cold: 1 row of 500 fp32 classes 3.2/5.0 us and 2.8/5.3, of 1001 3.9/5.8 and 2.9/4.9; 300 rows of
+    // 700 3.3/5.2 and 3.6/7.1, of 2000 5.0/6.9 and 4.3/6.8; where the warps of all rows fill the SMs 1000 rows of 4000 11.4/13.7 and 12.6/16.7, of 8000 16.6/19.6 and
+    // 14.5/18.8 (called one by one 16.6/19.5 and 16.4/20.5), of 16000 27.2/31.4 and 18.2/22.7; 4096 rows of 4000 24/29 and 40/54; in bf16 1000 rows of 16001 19.4/23.2 and 16.4/21.4 (in L2
+    // 12.7/16.7 and 12.7/18.2), of 32000 31.0/37.2 and 20.1/25.4.
     const bool narrow = a.split == 1 && (classes <= 768 || (rows > 4 * num_sms() && (long long)classes * size <= 32768));
 #define SB_LOGP(T, W) launch_logprobs<T, W>(a, logits, tokens, logprobs, entropy, top_logprobs, top_tokens, st)
     switch (in_type)

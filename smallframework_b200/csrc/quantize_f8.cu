@@ -8,7 +8,8 @@
 // Bound: memory (2 or 4 bytes read and one written an element), and close behind it the integer ALU (70 % of its slots at 8192x8192 bf16: unpacking, conversions,
 // packing).  16 lanes own 8 columns each of a block, so the largest magnitude of a row block is four shuffles away and nothing is read twice; four blocks a
 // lane are under way, and 16-bit values are compared two at a time as they are.
-// Measured on a B200: 8192x8192 bf16 40.5 us (5.0 TB/s, 31.2 at the copy rate), 5000x4112 fp32 in square blocks 19.2 us (5.4 TB/s, 15.9), 1x4096 2.0 us.
+// Measured on a B200, cold: 8192x8192 bf16 40.7 us (5.0 TB/s, 31.4 at the copy rate; in runs of a second 41.6), 5000x4112 fp32 in square blocks 19.3 us (5.3 TB/s, 15.9), 1x4096
+// 2.0 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -314,7 +315,8 @@ __global__ void __launch_bounds__(ROW_THREADS, TYPE == SMALL_B200_TYPE_F32 ? 4 :
 }
 
 // A CTA owns a square block: 16 lanes by 16 rows at a time, eight times, all of it in registers, 16-bit values as they are.  A block's loads and stores take turns,
-// so it is CTAs that hide them: 5000x4112 fp32 20.9 us with two an SM, 19.2 with three; 8192x8192 bf16 56 with two (values kept as floats), 45 with three, 41.5 with four.
+// so it is CTAs that hide them: 5000x4112 fp32 20.9 us with two an SM, 19.2 with three; 8192x8192 bf16 56 with two (values kept as floats), 45 with three, 41.2 with four.
+// The bounds cost a few registers in local memory (80 a thread and 28 bytes stored in fp32, 64 and 4 in 16 bits; rows that are read element by element 48 and 12).
 template <int TYPE, bool VEC>
 __global__ void __launch_bounds__(256, TYPE == SMALL_B200_TYPE_F32 ? 3 : 4)
     quantize_square_f8_kernel(const QuantArgs a, const void *in, uint8_t *out, float *scales)
