@@ -50,6 +50,8 @@ class FloatBuffer:
         return self.t.cpu().numpy()
 
     def swap(self, other):
+        if type(self) is not type(other) and isinstance(other, _NarrowBuffer):
+            raise ValueError(f"swap: {type(self).__name__} and {type(other).__name__}")
         self.__dict__, other.__dict__ = other.__dict__, self.__dict__
 
     @classmethod
@@ -100,7 +102,12 @@ class _NarrowBuffer:
         else:
             self.t = torch.empty(int(num_elts), dtype=self.dtype, device=device)
 
-    size, data, ptr, swap = FloatBuffer.size, FloatBuffer.data, FloatBuffer.ptr, FloatBuffer.swap
+    size, data, ptr = FloatBuffer.size, FloatBuffer.data, FloatBuffer.ptr
+
+    def swap(self, other):
+        if type(self) is not type(other):  # its elements would be counted by another size
+            raise ValueError(f"swap: {type(self).__name__} and {type(other).__name__}")
+        self.__dict__, other.__dict__ = other.__dict__, self.__dict__
 
     def numpy(self):
         return self.t.float().cpu().numpy()
